@@ -253,8 +253,10 @@ def _inputs(c, seed):
     table[rows, cols] = order[:rows.numel()]
     st["table"] = table
     if c["op"] == "plan":
-        st["free"] = order[rows.numel():].contiguous()
-        st["n_free"] = torch.tensor([st["free"].numel()], **i32)
+        # the free pages' stack: a buffer for every page of the pool, its first n_free entries valid
+        n_free = n_pages - rows.numel()
+        st["free"] = torch.cat((order[rows.numel():], torch.zeros(n_pages - n_free, **i32)))
+        st["n_free"] = torch.tensor([n_free], **i32)
         return st
     cu = [0]
     for n in new:
@@ -336,8 +338,8 @@ def _run_own(st):
     h = torch.cuda.current_stream().cuda_stream
     if c["op"] == "plan":
         s.kv8_plan(st["past"], st["new"], c["n_seq"], c["page"], st["table"], st["max_pages"], st["free"],
-                   st["n_free"], st["o_nfree"], st["n_tok"], st["o_cu"], st["o_len"], st["o_slot"], st["o_pos"],
-                   stream=h)
+                   st["n_pages"], st["n_free"], st["o_nfree"], st["n_tok"], st["o_cu"], st["o_len"], st["o_slot"],
+                   st["o_pos"], stream=h)
         return st["table"], st["o_cu"], st["o_len"], st["o_slot"], st["o_pos"], st["o_nfree"]
     if c["op"] == "store":
         s.kv8_store(st["cache"], st["type"], st["dk"], st["dv"], st["slot"], st["n_tok"], pos=st["pos"],
@@ -479,7 +481,7 @@ def run(state):
 def _exact_plan(st):
     page, n_seq = st["case"]["page"], st["case"]["n_seq"]
     table = st["table"].cpu().numpy().copy()
-    stack = st["free"].cpu().tolist()
+    stack = st["free"][:int(st["n_free"])].cpu().tolist()
     cu, slot, pos = [0], [], []
     for i in range(n_seq):
         p, n = st["past_host"][i], st["new_host"][i]
