@@ -79,6 +79,9 @@ SICU_API int sicu_status(int *flags);
 #define SICU_STATUS_WAIT_TIMEOUT 1
 #define SICU_STATUS_AR_TIMEOUT   2
 #define SICU_STATUS_BAD_ROW      4   /* sicu_row_to_f32_dev: a row id out of range */
+#define SICU_STATUS_NO_PAGES     8   /* sicu_kv8_plan: fewer free pages than the step needs */
+#define SICU_STATUS_BAD_PLAN    16   /* sicu_kv8_*: lengths, pages or slots on the device out of range */
+#define SICU_STATUS_NONFINITE   32   /* sicu_kv8_store: a K or V value that is not finite */
 
 /* Programmatic dependent launch for the matvec kernels (default off). When
  * on, a matvec may start streaming its weight blocks while earlier work in
@@ -478,6 +481,123 @@ SICU_API int sicu_attention_prompt(const float *dq, const float *dk, const float
                                    void *dv_cache, const float *dcos, const float *dsin, int64_t n_head,
                                    int64_t n_head_kv, int64_t head_dim, int64_t n_rot, int neox, int64_t n_ctx,
                                    int64_t pos0, int64_t m, float kq_scale, float *dout, void *stream);
+
+/* ---- paged 8-bit KV cache ----------------------------------------------------
+ * A cache for many requests at once, in pages of `page` tokens (16, 32, 64 or
+ * 128) that any request may own, held in 8 bits: one layer's codes and scales
+ *   k, v              int8 [n_pages][n_head_kv][page][head_dim]
+ *   k_scale, v_scale  f32  [n_pages][n_head_kv][page / 16]
+ * A stored value is code * scale, with one scale for each block of 16
+ * consecutive tokens and KV head. A request's block table lists its pages in
+ * order: position p lives in page table[p / page] at row p % page, which is
+ * slot table[p / page] * page + p % page. Pages are free or owned; the free
+ * ones are a stack free_pages[0 .. n_free) in a buffer of n_pages ids, taken
+ * from its end. All arrays are device memory unless said otherwise. head_dim
+ * is 64, 96, 128 or 256; codes 16-byte, scales 4-byte aligned. No counterpart
+ * in the reference, whose cache holds one sequence in f16 (src/engine.c:
+ * 336-366); sicu_attention_* serve that one.
+ *
+ * The calls neither allocate nor wait, and may be captured. Numbers that only
+ * the device knows are checked there: what is out of range is left out and
+ * SICU_STATUS_BAD_PLAN set; no call reads or writes outside the buffers it was
+ * described. */
+typedef struct sicu_kv8 {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t n_pages;
+    int32_t page;
+    int32_t n_head_kv;
+    int32_t head_dim;
+} sicu_kv8;
+/* RoPE tables cos, sin [rows][n_rot / 2] by position (16-byte aligned, n_rot
+ * a multiple of 8 up to head_dim): pairs (2j, 2j+1), or (j, j + head_dim / 2)
+ * when neox != 0; x0' = x0 c - x1 s, x1' = x0 s + x1 c with every product and
+ * sum rounded to f32 on its own. Channels past n_rot are unchanged. */
+typedef struct sicu_rope_tables {
+    const float *cos, *sin;
+    int64_t rows;
+    int32_t n_rot;
+    int32_t neox;
+} sicu_rope_tables;
+/* A step's block tables and slot map: request i of n_seq (up to 8192) holds
+ * past[i] tokens and adds fresh[i] (0 allowed). Appends the pages it needs to
+ * its row of table [n_seq][max_pages], taken from the stack's top in request
+ * order, and writes cu [n_seq + 1] (tokens added by the requests before each
+ * one: where its rows start in the packed activations), len [n_seq] (past +
+ * fresh), and for each packed token its slot and position (slot 16-byte, pos
+ * 16-byte aligned, n_tok entries; -1 and 0 past the last token). n_free_out
+ * receives the new stack height. len may be past and n_free_out n_free. A step
+ * that does not fit places nothing (cu all 0, slots all -1, len = past,
+ * n_free_out = n_free): SICU_STATUS_NO_PAGES when the stack is too short,
+ * SICU_STATUS_BAD_PLAN for a negative length, a request past max_pages or more
+ * than n_tok tokens. */
+SICU_API int sicu_kv8_plan(const int32_t *past, const int32_t *fresh, int64_t n_seq, int32_t page, int32_t *table,
+                           int64_t max_pages, const int32_t *free_pages, int64_t n_pages, const int32_t *n_free,
+                           int32_t *n_free_out, int64_t n_tok, int32_t *cu, int32_t *len, int64_t *slot, int32_t *pos,
+                           void *stream);
+/* Returns the pages of every request with drop[i] != 0 to the stack and sets
+ * its len[i] to 0. */
+SICU_API int sicu_kv8_release(const int32_t *drop, int32_t *len, int64_t n_seq, int32_t page, const int32_t *table,
+                              int64_t max_pages, int32_t *free_pages, int64_t n_pages, int32_t *n_free, void *stream);
+/* Stores n_tok tokens' K and V rows (type SICU_T_F32 or SICU_T_F16,
+ * n_head_kv * head_dim values each, k_stride / v_stride elements between
+ * tokens, rows 16-byte aligned) at their slots, K rotated at pos[t] first when
+ * rope is given (NULL: not). Tokens of one 16-token block are adjacent and in
+ * ascending order, as sicu_kv8_plan lists them, and rows of a block before the
+ * first of them are valid. A negative slot's token is skipped. A block's scale
+ * becomes s = max(s, max|x| / 127) over the rows given (from 0 when they begin
+ * the block), rows stored earlier are requantized when it grows (rint(code *
+ * (s_old * (1 / s)))), and each row becomes rint(x * (1 / s)). Magnitudes
+ * below 2^-112 count as 0. A value that is not finite does not enter the scale:
+ * it is stored as 0 (NaN) or +-127 (infinities) and SICU_STATUS_NONFINITE set. */
+SICU_API int sicu_kv8_store(const sicu_kv8 *cache, uint32_t type, const void *dk, const void *dv, int64_t k_stride,
+                            int64_t v_stride, const int64_t *slot, const int32_t *pos, const sicu_rope_tables *rope,
+                            int64_t n_tok, void *stream);
+/* The stored rows of n_tok slots as values code * scale in f32 (rounded once
+ * to f16 for SICU_T_F16): dk, dv [n_tok][n_head_kv * head_dim], 16-byte
+ * aligned; zero rows for negative slots. */
+SICU_API int sicu_kv8_load(const sicu_kv8 *cache, uint32_t type, const int64_t *slot, int64_t n_tok, void *dk, void *dv,
+                           void *stream);
+/* Attention of a step's new tokens over the cache. Request i's rows are the
+ * packed tokens cu[i] .. cu[i + 1), the last positions of its len[i]
+ * (stored already, its own included); query head h reads KV head
+ * h / (n_head / n_head_kv). For row p and key j
+ *   z = scale * (q . k_j);  z = cap * tanh(z / cap) when cap > 0;
+ *   z -= slopes[h] * |p - j| when slopes is given
+ * over the visible keys: j <= p, or j < prefix[i] when given (a prefix that
+ * sees itself both ways); j > p - window when window > 0; j >= first[i] when
+ * given (older tokens were evicted; their pages are not read). out = sum of
+ * softmax(z)_j v_j; a row that sees no key is 0. q and out: type SICU_T_F32 or
+ * SICU_T_F16, n_head * head_dim values per token, q_stride / out_stride
+ * elements apart, 16-byte aligned; q is rotated at its position when rope is
+ * given and left as it is in memory. Sums and maxima are f32; f32 results
+ * agree with a computation in f32, f16 ones are rounded once at the end (the
+ * softmax weights pass through f16 in between). max_new and max_len bound the
+ * requests' new tokens and lengths (host values). */
+typedef struct sicu_kv8_attn {
+    uint32_t type;
+    int32_t n_head;
+    int64_t n_tok;                /* rows in q and out */
+    int64_t q_stride, out_stride; /* 0: n_head * head_dim */
+    const int32_t *table;         /* [n_seq][max_pages] */
+    int64_t max_pages;
+    const int32_t *len;           /* [n_seq] */
+    const int32_t *cu;            /* [n_seq + 1] */
+    int64_t n_seq;
+    int64_t max_new, max_len;
+    float scale;
+    float cap;                    /* 0: none */
+    const float *slopes;          /* [n_head] or NULL */
+    int64_t window;               /* 0: none */
+    const int32_t *prefix;        /* [n_seq] or NULL */
+    const int32_t *first;         /* [n_seq] or NULL */
+    const sicu_rope_tables *rope; /* host struct, or NULL */
+} sicu_kv8_attn;
+/* Workspace bytes for a call with these sizes (pointers are not looked at);
+ * ws is 16-byte aligned and belongs to the call until it has run. */
+SICU_API int sicu_kv8_attention_ws(const sicu_kv8 *cache, const sicu_kv8_attn *a, size_t *bytes);
+SICU_API int sicu_kv8_attention(const sicu_kv8 *cache, const sicu_kv8_attn *a, const void *dq, void *dout, void *ws,
+                                size_t ws_bytes, void *stream);
 
 /* ---- dequantisation --------------------------------------------------------
  * Rows rows[0..nrows) (host array) of W into dout[nrows][n_in] f32, reference

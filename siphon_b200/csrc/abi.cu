@@ -1267,4 +1267,223 @@ int sicu_row_to_f32(uint32_t wtype, const void *dw, int64_t n_in, const int64_t 
     return SICU_OK;
 }
 
+// ---- paged 8-bit KV cache ------------------------------------------------------
+static int page_shift(int32_t page) {
+    return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
+}
+
+static int check_kv8(const char *what, const sicu_kv8 *c, bool pointers, Kv8Dev &d) {
+    if (!c) return fail(SICU_EINVAL, "%s: null cache", what);
+    const int sh = page_shift(c->page);
+    if (sh < 0) return fail(SICU_EINVAL, "%s: pages of %d tokens (16, 32, 64 or 128)", what, c->page);
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(SICU_ENOTSUP, "%s: head size %d (64, 96, 128 or 256)", what, c->head_dim);
+    if (c->n_head_kv <= 0 || c->n_head_kv > 4096) return fail(SICU_EINVAL, "%s: %d KV heads", what, c->n_head_kv);
+    if (c->n_pages <= 0 || c->n_pages > INT32_MAX) return fail(SICU_EINVAL, "%s: %lld pages", what, (long long)c->n_pages);
+    if (pointers) {
+        if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(SICU_EINVAL, "%s: null cache pointer", what);
+        if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+            return fail(SICU_EINVAL, "%s: codes must be 16-byte and scales 4-byte aligned", what);
+    }
+    d.k = c->k;
+    d.v = c->v;
+    d.ks = c->k_scale;
+    d.vs = c->v_scale;
+    d.n_pages = c->n_pages;
+    d.page = c->page;
+    d.page_shift = sh;
+    d.hkv = c->n_head_kv;
+    d.hd = c->head_dim;
+    return SICU_OK;
+}
+
+static int check_rope_tables(const char *what, const sicu_rope_tables *r, int head_dim, RopeDev &d) {
+    d = RopeDev{};
+    if (!r) return SICU_OK;
+    if (r->n_rot < 0 || r->n_rot > head_dim || r->n_rot % 8)
+        return fail(SICU_EINVAL, "%s: %d rotated channels of %d (a multiple of 8)", what, r->n_rot, head_dim);
+    if (r->n_rot == 0) return SICU_OK;
+    if (r->rows <= 0) return fail(SICU_EINVAL, "%s: RoPE tables of %lld positions", what, (long long)r->rows);
+    if (!r->cos || !r->sin) return fail(SICU_EINVAL, "%s: null RoPE table", what);
+    if (!aligned(r->cos, 16) || !aligned(r->sin, 16)) return fail(SICU_EINVAL, "%s: RoPE tables must be 16-byte aligned", what);
+    d.cs = r->cos;
+    d.sn = r->sin;
+    d.rows = r->rows;
+    d.half = r->n_rot / 2;
+    d.neox = r->neox ? 1 : 0;
+    return SICU_OK;
+}
+
+// element size of an activation type, 0 for others
+static int64_t act_size(uint32_t type) { return type == T_F32 ? 4 : type == T_F16 ? 2 : 0; }
+
+// rows of `width` values `stride` elements apart (0: packed)
+static int check_rows(const char *what, const void *p, int64_t size, int64_t width, int64_t &stride) {
+    if (stride == 0) stride = width;
+    if (stride < width) return fail(SICU_EINVAL, "%s: row stride %lld below %lld", what, (long long)stride, (long long)width);
+    if (stride > ((int64_t)1 << 40)) return fail(SICU_EINVAL, "%s: row stride %lld", what, (long long)stride);
+    if (!p) return fail(SICU_EINVAL, "%s: null pointer", what);
+    if (!aligned(p, 16) || stride * size % 16) return fail(SICU_EINVAL, "%s: rows must be 16-byte aligned", what);
+    return SICU_OK;
+}
+
+int sicu_kv8_plan(const int32_t *past, const int32_t *fresh, int64_t n_seq, int32_t page, int32_t *table,
+                  int64_t max_pages, const int32_t *free_pages, int64_t n_pages, const int32_t *n_free,
+                  int32_t *n_free_out, int64_t n_tok, int32_t *cu, int32_t *len, int64_t *slot, int32_t *pos,
+                  void *stream) {
+    const int sh = page_shift(page);
+    if (sh < 0) return fail(SICU_EINVAL, "kv8 plan: pages of %d tokens (16, 32, 64 or 128)", page);
+    if (n_seq < 1 || n_seq > KV8_MAX_SEQ) return fail(SICU_EINVAL, "kv8 plan: %lld requests (1..%d)", (long long)n_seq, KV8_MAX_SEQ);
+    if (max_pages < 1 || max_pages > (INT32_MAX >> sh) || n_pages < 1 || n_pages > INT32_MAX || n_tok < 0 ||
+        n_tok > INT32_MAX - 4)
+        return fail(SICU_EINVAL, "kv8 plan: bad size (max_pages=%lld, n_pages=%lld, n_tok=%lld)", (long long)max_pages,
+                    (long long)n_pages, (long long)n_tok);
+    if (!past || !fresh || !table || !free_pages || !n_free || !n_free_out || !cu || !len || (n_tok && (!slot || !pos)))
+        return fail(SICU_EINVAL, "kv8 plan: null pointer");
+    if (!aligned(slot, 16) || !aligned(pos, 16)) return fail(SICU_EINVAL, "kv8 plan: slots and positions must be 16-byte aligned");
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    const Kv8PlanLaunch L{past, fresh, (int)n_seq, sh, (int)max_pages, table, free_pages, n_pages, n_free, n_free_out,
+                          n_tok, cu, len, slot, pos, ds->status};
+    if (launch_kv8_plan(L, (cudaStream_t)stream)) return cuda_fail(cudaGetLastError(), "kv8 plan launch");
+    return SICU_OK;
+}
+
+int sicu_kv8_release(const int32_t *drop, int32_t *len, int64_t n_seq, int32_t page, const int32_t *table,
+                     int64_t max_pages, int32_t *free_pages, int64_t n_pages, int32_t *n_free, void *stream) {
+    const int sh = page_shift(page);
+    if (sh < 0) return fail(SICU_EINVAL, "kv8 release: pages of %d tokens (16, 32, 64 or 128)", page);
+    if (n_seq < 1 || n_seq > KV8_MAX_SEQ) return fail(SICU_EINVAL, "kv8 release: %lld requests (1..%d)", (long long)n_seq, KV8_MAX_SEQ);
+    if (max_pages < 1 || max_pages > (INT32_MAX >> sh) || n_pages < 1 || n_pages > INT32_MAX)
+        return fail(SICU_EINVAL, "kv8 release: bad size (max_pages=%lld, n_pages=%lld)", (long long)max_pages, (long long)n_pages);
+    if (!drop || !len || !table || !free_pages || !n_free) return fail(SICU_EINVAL, "kv8 release: null pointer");
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    if (launch_kv8_release(drop, len, (int)n_seq, sh, table, max_pages, free_pages, n_pages, n_free, ds->status,
+                           (cudaStream_t)stream))
+        return cuda_fail(cudaGetLastError(), "kv8 release launch");
+    return SICU_OK;
+}
+
+int sicu_kv8_store(const sicu_kv8 *cache, uint32_t type, const void *dk, const void *dv, int64_t k_stride,
+                   int64_t v_stride, const int64_t *slot, const int32_t *pos, const sicu_rope_tables *rope,
+                   int64_t n_tok, void *stream) {
+    Kv8Dev c;
+    RopeDev r;
+    if (int rc = check_kv8("kv8 store", cache, true, c)) return rc;
+    const int64_t size = act_size(type), width = (int64_t)c.hkv * c.hd;
+    if (!size) return fail(SICU_ENOTSUP, "kv8 store: unsupported activation type %s (%u)", tname(type), type);
+    if (int rc = check_rope_tables("kv8 store", rope, c.hd, r)) return rc;
+    if (n_tok < 0 || n_tok > INT32_MAX) return fail(SICU_EINVAL, "kv8 store: %lld tokens", (long long)n_tok);
+    if (n_tok == 0) return current_ok();
+    if (int rc = check_rows("kv8 store K", dk, size, width, k_stride)) return rc;
+    if (int rc = check_rows("kv8 store V", dv, size, width, v_stride)) return rc;
+    if (!slot || (r.half && !pos)) return fail(SICU_EINVAL, "kv8 store: null slots or positions");
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    if (launch_kv8_store(c, type == T_F16, dk, dv, k_stride, v_stride, slot, pos, r, n_tok, ds->sms, ds->status,
+                         (cudaStream_t)stream))
+        return cuda_fail(cudaGetLastError(), "kv8 store launch");
+    return SICU_OK;
+}
+
+int sicu_kv8_load(const sicu_kv8 *cache, uint32_t type, const int64_t *slot, int64_t n_tok, void *dk, void *dv,
+                  void *stream) {
+    Kv8Dev c;
+    if (int rc = check_kv8("kv8 load", cache, true, c)) return rc;
+    if (!act_size(type)) return fail(SICU_ENOTSUP, "kv8 load: unsupported activation type %s (%u)", tname(type), type);
+    if (n_tok < 0 || n_tok > INT32_MAX) return fail(SICU_EINVAL, "kv8 load: %lld tokens", (long long)n_tok);
+    if (n_tok == 0) return current_ok();
+    if (!slot || !dk || !dv) return fail(SICU_EINVAL, "kv8 load: null pointer");
+    if (!aligned(dk, 16) || !aligned(dv, 16)) return fail(SICU_EINVAL, "kv8 load: rows must be 16-byte aligned");
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    if (launch_kv8_load(c, type == T_F16, slot, n_tok, dk, dv, ds->status, (cudaStream_t)stream))
+        return cuda_fail(cudaGetLastError(), "kv8 load launch");
+    return SICU_OK;
+}
+
+// sizes and scalars of an attention call (no pointers)
+static int check_kv8_attn(const Kv8Dev &c, const sicu_kv8_attn *a, Kv8AttnDev &d) {
+    if (!a) return fail(SICU_EINVAL, "kv8 attention: null description");
+    if (!act_size(a->type)) return fail(SICU_ENOTSUP, "kv8 attention: unsupported activation type %s (%u)", tname(a->type), a->type);
+    if (a->n_head <= 0 || a->n_head > 65536 || a->n_head % c.hkv)
+        return fail(SICU_EINVAL, "kv8 attention: %d heads over %d KV heads", a->n_head, c.hkv);
+    if (a->n_seq < 0 || a->n_seq > KV8_MAX_SEQ) return fail(SICU_EINVAL, "kv8 attention: %lld requests (0..%d)", (long long)a->n_seq, KV8_MAX_SEQ);
+    if (a->n_tok < 0 || a->n_tok > INT32_MAX - 64) return fail(SICU_EINVAL, "kv8 attention: %lld tokens", (long long)a->n_tok);
+    if (a->max_pages < 1 || a->max_len < 0 || a->max_len > INT32_MAX - 1024 || a->max_pages > (INT32_MAX >> c.page_shift) ||
+        a->max_len > a->max_pages << c.page_shift)
+        return fail(SICU_EINVAL, "kv8 attention: lengths up to %lld in %lld pages of %d", (long long)a->max_len,
+                    (long long)a->max_pages, c.page);
+    if (a->max_new < 0 || a->max_new > a->n_tok || a->max_new > a->max_len)
+        return fail(SICU_EINVAL, "kv8 attention: up to %lld new tokens of %lld", (long long)a->max_new, (long long)a->n_tok);
+    if (a->max_new * (a->n_head / c.hkv) > INT32_MAX - 1024) return fail(SICU_EINVAL, "kv8 attention: too many rows");
+    if (a->window < 0) return fail(SICU_EINVAL, "kv8 attention: negative window");
+    if (!(a->cap >= 0.0f) || !(a->cap <= 1e30f) || (a->cap > 0.0f && a->cap < 1e-30f))
+        return fail(SICU_EINVAL, "kv8 attention: cap %g", (double)a->cap);
+    d = Kv8AttnDev{};
+    d.n_tok = (int)a->n_tok;
+    d.n_head = a->n_head;
+    d.n_seq = (int)a->n_seq;
+    d.max_pages = a->max_pages;
+    d.max_new = (int)a->max_new;
+    d.max_len = (int)a->max_len;
+    d.scale = a->scale;
+    d.cap = a->cap;
+    d.window = a->window > a->max_len ? 0 : (int)a->window;
+    return SICU_OK;
+}
+
+static int kv8_sms(int &sms) {
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    sms = ds->sms;
+    return SICU_OK;
+}
+
+int sicu_kv8_attention_ws(const sicu_kv8 *cache, const sicu_kv8_attn *a, size_t *bytes) {
+    Kv8Dev c;
+    Kv8AttnDev d;
+    if (!bytes) return fail(SICU_EINVAL, "kv8 attention: null out pointer");
+    if (int rc = check_kv8("kv8 attention", cache, false, c)) return rc;
+    if (int rc = check_kv8_attn(c, a, d)) return rc;
+    int sms;
+    if (int rc = kv8_sms(sms)) return rc;
+    *bytes = d.n_seq && d.max_new ? kv8_attn_workspace(c, d, a->type == T_F16, sms) : 0;
+    return SICU_OK;
+}
+
+int sicu_kv8_attention(const sicu_kv8 *cache, const sicu_kv8_attn *a, const void *dq, void *dout, void *ws,
+                       size_t ws_bytes, void *stream) {
+    Kv8Dev c;
+    Kv8AttnDev d;
+    if (int rc = check_kv8("kv8 attention", cache, true, c)) return rc;
+    if (int rc = check_kv8_attn(c, a, d)) return rc;
+    if (int rc = check_rope_tables("kv8 attention", a->rope, c.hd, d.rope)) return rc;
+    if (d.n_seq == 0 || d.max_new == 0) return current_ok();
+    const int64_t size = act_size(a->type), width = (int64_t)a->n_head * c.hd;
+    d.q_stride = a->q_stride;
+    d.out_stride = a->out_stride;
+    if (int rc = check_rows("kv8 attention q", dq, size, width, d.q_stride)) return rc;
+    if (int rc = check_rows("kv8 attention out", dout, size, width, d.out_stride)) return rc;
+    if (!a->table || !a->len || !a->cu) return fail(SICU_EINVAL, "kv8 attention: null table, lengths or cu");
+    DevState *ds;
+    if (int rc = current(ds)) return rc;
+    const size_t need = kv8_attn_workspace(c, d, a->type == T_F16, ds->sms);
+    if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
+        return fail(SICU_EINVAL, "kv8 attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);
+    d.q = dq;
+    d.out = dout;
+    d.table = a->table;
+    d.len = a->len;
+    d.cu = a->cu;
+    d.slopes = a->slopes;
+    d.prefix = a->prefix;
+    d.first = a->first;
+    d.status = ds->status;
+    if (launch_kv8_attention(c, d, a->type == T_F16, ws, ds->sms, (cudaStream_t)stream))
+        return cuda_fail(cudaGetLastError(), "kv8 attention launch");
+    return SICU_OK;
+}
+
 }  // extern "C"

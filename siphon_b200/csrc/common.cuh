@@ -26,6 +26,9 @@ constexpr int STATUS_WAIT_TIMEOUT = 1;
 // broken by an earlier failure
 constexpr int STATUS_AR_TIMEOUT = 2;
 constexpr int STATUS_BAD_ROW = 4;    // a row id read from device memory was out of range
+// paged 8-bit KV cache: too few free pages for a step; lengths, pages or slots
+// read from device memory out of range; a K or V value that is not finite
+constexpr int STATUS_NO_PAGES = 8, STATUS_BAD_PLAN = 16, STATUS_NONFINITE = 32;
 
 // ---- f16 ---------------------------------------------------------------------
 // f16 -> f32 is exact in hardware for every finite half and inf.

@@ -1,0 +1,463 @@
+// The paged 8-bit KV cache outside its attention: block tables and slot maps
+// from request lengths, release of a request's pages, the quantizing store of
+// new tokens (with RoPE), and the read-back of stored rows.
+#include "kv8.cuh"
+
+namespace sicu {
+namespace {
+
+// ---- block tables and slot maps ----------------------------------------------------
+//
+// take_i = ceil((past_i + new_i) / page) - ceil(past_i / page) pages are taken
+// from the top of the free stack in request order; cu is the exclusive prefix
+// sum of new_i; token t of request i at position p has slot
+// table[i][p / page] * page + p % page. All integers, a few bytes per request
+// and 12 per token: a step is bound by latency (one scan, one search), not by
+// bytes. One launch: every CTA of one cluster scans all requests itself into
+// shared memory (a scan of 1024 requests is cheaper than handing results
+// over), the cluster barrier separates every read of the inputs from the first
+// write (outputs may replace inputs in place), and the pages and tokens are
+// then dealt over all threads, each finding its request by binary search in
+// shared memory. The slots of new pages come from the stack itself, not from
+// the table another CTA may still be writing.
+constexpr int PLAN_THREADS = 1024;
+
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// inclusive scan of two values over the CTA
+__device__ void block_scan2(int64_t &a, int64_t &b, int64_t (*part)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    a = warp_scan(a, lane);
+    b = warp_scan(b, lane);
+    if (lane == 31) {
+        part[warp][0] = a;
+        part[warp][1] = b;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const bool in = lane < (int)(blockDim.x >> 5);
+        const int64_t x = warp_scan(in ? part[lane][0] : 0, lane), y = warp_scan(in ? part[lane][1] : 0, lane);
+        if (in) {
+            part[lane][0] = x;
+            part[lane][1] = y;
+        }
+    }
+    __syncthreads();
+    if (warp > 0) {
+        a += part[warp - 1][0];
+        b += part[warp - 1][1];
+    }
+}
+
+// the last i in [0, n) with start[i] <= x, where start[0] = 0 and x < start[n]
+__device__ __forceinline__ int find(const int32_t *start, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) kv8_plan_kernel(Kv8PlanLaunch L) {
+    extern __shared__ int32_t plan_sm[];
+    int32_t *cu = plan_sm, *tk = plan_sm + L.n_seq + 1, *past = tk + L.n_seq + 1;
+    __shared__ int64_t part[PLAN_THREADS / 32][2];
+    const int tid = threadIdx.x, n = L.n_seq, sh = L.page_shift, pm = (1 << sh) - 1;
+    const int64_t cap = (int64_t)L.max_pages << sh;
+    int64_t base_new = 0, base_take = 0;
+    bool bad = false;
+    for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+        const int i = i0 + tid;
+        int64_t add = 0, take = 0;
+        if (i < n) {
+            const int64_t p = L.past[i], f = L.fresh[i];
+            past[i] = (int)p;
+            if (p < 0 || f < 0 || p + f > cap) bad = true;
+            else {
+                add = f;
+                take = ((p + f + pm) >> sh) - ((p + pm) >> sh);
+            }
+        }
+        int64_t a = add, t = take;
+        block_scan2(a, t, part);
+        a += base_new;
+        t += base_take;
+        if (i < n) {
+            // totals past the limits below are refused before these are used
+            cu[i] = (int)(a - add);
+            tk[i] = (int)(t - take);
+        }
+        base_new += part[PLAN_THREADS / 32 - 1][0];
+        base_take += part[PLAN_THREADS / 32 - 1][1];
+        __syncthreads();
+    }
+    const int64_t n_free = *L.n_free;
+    bad = __syncthreads_or(bad || n_free < 0 || n_free > L.n_pages || base_new > L.max_tok);
+    const bool none = !bad && base_take > n_free;
+    if (tid == 0) {
+        cu[n] = (int)base_new;
+        tk[n] = (int)base_take;
+    }
+    cluster_sync();                       // every input is read before any output is written
+    const int gt = blockIdx.x * PLAN_THREADS + tid, gn = gridDim.x * PLAN_THREADS;
+    if (bad || none) {
+        // a step that cannot be placed places nothing
+        for (int i = gt; i <= n; i += gn) {
+            L.cu[i] = 0;
+            if (i < n) L.len[i] = past[i];
+        }
+        for (int64_t t = gt; t < L.max_tok; t += gn) {
+            L.slot[t] = -1;
+            L.pos[t] = 0;
+        }
+        if (gt == 0) {
+            *L.n_free_out = (int)n_free;
+            atomicOr(L.status, bad ? STATUS_BAD_PLAN : STATUS_NO_PAGES);
+        }
+        return;
+    }
+    for (int i = gt; i <= n; i += gn) {
+        L.cu[i] = cu[i];
+        if (i < n) L.len[i] = past[i] + cu[i + 1] - cu[i];
+    }
+    if (gt == 0) *L.n_free_out = (int)(n_free - base_take);
+    for (int j = gt; j < tk[n]; j += gn) {
+        const int i = find(tk, n, j);
+        const int col = ((past[i] + pm) >> sh) + j - tk[i];
+        L.table[(int64_t)i * L.max_pages + col] = L.free_pages[n_free - 1 - j];
+    }
+    const int n_tok = cu[n];
+    for (int64_t t4 = 4 * (int64_t)gt; t4 < L.max_tok; t4 += 4 * (int64_t)gn) {
+        int64_t s[4];
+        int32_t ps[4];
+        int i = t4 < n_tok ? find(cu, n, (int)t4) : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int t = (int)t4 + e;
+            s[e] = -1;
+            ps[e] = 0;
+            if (t4 + e < n_tok) {
+                while (t >= cu[i + 1]) ++i;
+                const int p = past[i] + t - cu[i], col = p >> sh, held = (past[i] + pm) >> sh;
+                const int page = col < held ? L.table[(int64_t)i * L.max_pages + col]
+                                            : L.free_pages[n_free - 1 - (tk[i] + col - held)];
+                s[e] = ((int64_t)page << sh) + (p & pm);
+                ps[e] = p;
+            }
+        }
+        if (t4 + 4 <= L.max_tok) {
+            reinterpret_cast<longlong2 *>(L.slot + t4)[0] = make_longlong2(s[0], s[1]);
+            reinterpret_cast<longlong2 *>(L.slot + t4)[1] = make_longlong2(s[2], s[3]);
+            *reinterpret_cast<int4 *>(L.pos + t4) = make_int4(ps[0], ps[1], ps[2], ps[3]);
+        } else {
+            for (int e = 0; t4 + e < L.max_tok; ++e) {
+                L.slot[t4 + e] = s[e];
+                L.pos[t4 + e] = ps[e];
+            }
+        }
+    }
+}
+
+// Pages of the requests with drop[i] != 0 go back on the stack in request and
+// page order; their lengths become 0. One CTA: the counts are small and the
+// stack's new top depends on all of them.
+__global__ void __launch_bounds__(PLAN_THREADS) kv8_release_kernel(const int32_t *drop, int32_t *len, int n, int sh,
+                                                                   const int32_t *table, int64_t max_pages,
+                                                                   int32_t *free_pages, int64_t n_pages,
+                                                                   int32_t *n_free, int *status) {
+    extern __shared__ int32_t rel_sm[];     // rel_sm[i]: pages released before request i
+    __shared__ int64_t part[PLAN_THREADS / 32][2];
+    const int tid = threadIdx.x, pm = (1 << sh) - 1;
+    int64_t base = 0, zero;
+    bool bad = false;
+    for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+        const int i = i0 + tid;
+        int64_t cnt = 0;
+        if (i < n && drop[i]) {
+            const int64_t l = len[i];
+            if (l < 0 || l > (max_pages << sh)) bad = true;
+            else cnt = (l + pm) >> sh;
+        }
+        int64_t a = cnt;
+        zero = 0;
+        block_scan2(a, zero, part);
+        if (i < n) rel_sm[i] = (int)(base + a - cnt);
+        base += part[PLAN_THREADS / 32 - 1][0];
+        __syncthreads();
+    }
+    const int64_t top = *n_free;
+    bad = __syncthreads_or(bad || top < 0 || top + base > n_pages);
+    if (bad) {
+        if (tid == 0) atomicOr(status, STATUS_BAD_PLAN);
+        return;
+    }
+    if (tid == 0) rel_sm[n] = (int)base;
+    __syncthreads();
+    for (int j = tid; j < (int)base; j += PLAN_THREADS) {
+        const int i = find(rel_sm, n, j);
+        free_pages[top + j] = table[(int64_t)i * max_pages + (j - rel_sm[i])];
+    }
+    for (int i = tid; i < n; i += PLAN_THREADS)
+        if (drop[i]) len[i] = 0;
+    if (tid == 0) *n_free = (int)(top + base);
+}
+
+// ---- store ---------------------------------------------------------------------------
+//
+// A block's scale is the largest |x| it was given over 127; code = rne(x /
+// scale). Rows appended to a block that already holds some may need a larger
+// scale: the codes in place are then requantized to it (rne(code * old / new)),
+// each at most once per doubling of the scale in practice. One warp owns one
+// (block, KV head, K or V): it loads the block's new rows once into registers,
+// rotates K, reduces the magnitude, and writes codes, so a step reads its
+// inputs once and writes one byte per element; nothing is shared between warps
+// and the result does not depend on their order. Bound by DRAM bytes for
+// prompts and by one load-reduce-store latency for single tokens.
+constexpr int STORE_WARPS = 4;
+// smallest magnitude worth a scale: below it 1 / scale would leave f32's range
+constexpr float KV8_TINY = 1.92592994e-34f;     // 2^-112
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(STORE_WARPS * 32) kv8_store_kernel(Kv8Dev c, const T *k, const T *v, int64_t k_stride,
+                                                                     int64_t v_stride, const int64_t *slot,
+                                                                     const int32_t *pos, RopeDev rope, int64_t n_tok,
+                                                                     int chunk, int *status) {
+    constexpr int OCTS = HD / 8;                 // 8-channel pieces per row
+    constexpr int IT = KV8_BLOCK * OCTS / 32;    // pieces per lane
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+    const int64_t c0 = (int64_t)blockIdx.x * chunk;
+    // tokens of the chunk that open a run of rows for one block
+    const int64_t t = c0 + lane;
+    bool opens = false;
+    if (lane < chunk && t < n_tok) {
+        const int64_t s = slot[t];
+        if (s >= 0) opens = t == 0 || slot[t - 1] < 0 || (slot[t - 1] >> 4) != (s >> 4);
+    }
+    const uint32_t starts = __ballot_sync(0xffffffffu, opens);
+    const int jobs = 2 * __popc(starts);
+    for (int j = warp; j < jobs; j += STORE_WARPS) {
+        const bool is_v = j & 1;
+        const int64_t r0 = c0 + __fns(starts, 0, (j >> 1) + 1);
+        // the run: rows r0 .. r0 + n - 1 in one block
+        int64_t s = -1;
+        if (lane < KV8_BLOCK && r0 + lane < n_tok) s = slot[r0 + lane];
+        const int64_t s0 = __shfl_sync(0xffffffffu, s, 0);
+        const uint32_t same = __ballot_sync(0xffffffffu, s >= 0 && (s >> 4) == (s0 >> 4));
+        const int n = __ffs(~same) - 1;
+        const int off = (int)(s & (KV8_BLOCK - 1)), lead = __shfl_sync(0xffffffffu, off, 0);
+        const int64_t pg = s0 >> c.page_shift;
+        if (pg >= c.n_pages) {
+            if (lane == 0) atomicOr(status, STATUS_BAD_PLAN);
+            continue;
+        }
+        const int64_t blk = kv8_block(c, (int)pg, head, (int)(s0 & (c.page - 1)) >> 4);
+        const T *src = (is_v ? v : k) + r0 * (is_v ? v_stride : k_stride) + (int64_t)head * HD;
+        const int64_t stride = is_v ? v_stride : k_stride;
+        const int neox = is_v ? 0 : rope.neox;
+        float *scale = (is_v ? c.vs : c.ks) + blk;
+        int8_t *codes = (is_v ? c.v : c.k) + blk * (KV8_BLOCK * HD);
+        const float before = lead > 0 ? *scale : 0.0f;
+        Oct x[IT];
+        float amax = 0.0f;
+        bool odd = false;
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
+            if (row < n) {
+                load4(src + row * stride + oct_a(o, neox), x[it].a);
+                load4(src + row * stride + oct_b(o, HD, neox), x[it].b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[it].a[e] = x[it].b[e] = 0.0f;
+            }
+        }
+        if (!is_v && rope.half) {
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
+                if (row < n) {
+                    const int64_t p = pos[r0 + row];
+                    if (p >= 0 && p < rope.rows) rope_oct(x[it], rope, p, o);
+                    else if (o == 0) atomicOr(status, STATUS_BAD_PLAN);
+                }
+            }
+        }
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float ma = fabsf(x[it].a[e]), mb = fabsf(x[it].b[e]);
+                const bool fa = ma <= 3.402823466e38f, fb = mb <= 3.402823466e38f;
+                odd |= !fa || !fb;
+                amax = fmaxf(amax, fmaxf(fa ? ma : 0.0f, fb ? mb : 0.0f));
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        const float sc = fmaxf(before, amax >= KV8_TINY ? __fdiv_rn(amax, 127.0f) : 0.0f);
+        const float inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
+        if (__any_sync(0xffffffffu, odd) && lane == 0) atomicOr(status, STATUS_NONFINITE);
+        if (sc > before && lead > 0) {
+            // rows stored earlier: their codes at the larger scale
+            const float r = __fmul_rn(before, inv);
+            uint32_t *w = reinterpret_cast<uint32_t *>(codes);
+            for (int i = lane; i < lead * (HD / 4); i += 32) {
+                const uint32_t u = w[i];
+                uint32_t o = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int q = (int)(int8_t)(u >> (8 * b));
+                    o |= ((uint32_t)__float2int_rn(__fmul_rn((float)q, r)) & 0xffu) << (8 * b);
+                }
+                w[i] = o;
+            }
+        }
+        if (lane == 0) *scale = sc;
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
+            // one row per lane below: the row's own offset in its block
+            const int at = __shfl_sync(0xffffffffu, off, row);
+            if (row < n) {
+                uint32_t wa = 0, wb = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // a NaN becomes 0, an infinity the largest code of its sign
+                    const int qa = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].a[e], inv))));
+                    const int qb = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].b[e], inv))));
+                    wa |= ((uint32_t)qa & 0xffu) << (8 * e);
+                    wb |= ((uint32_t)qb & 0xffu) << (8 * e);
+                }
+                int8_t *dst = codes + at * HD;
+                if (neox) {
+                    *reinterpret_cast<uint32_t *>(dst + oct_a(o, 1)) = wa;
+                    *reinterpret_cast<uint32_t *>(dst + oct_b(o, HD, 1)) = wb;
+                } else {
+                    *reinterpret_cast<uint2 *>(dst + 8 * o) = make_uint2(wa, wb);
+                }
+            }
+        }
+    }
+}
+
+// ---- load ----------------------------------------------------------------------------
+// Rows of the cache as values: code * scale. 16 codes per thread; bound by the
+// bytes of the values written.
+template <typename T>
+__global__ void __launch_bounds__(256) kv8_load_kernel(Kv8Dev c, const int64_t *slot, int64_t n_tok, T *k, T *v,
+                                                       int *status) {
+    const int pieces = c.hkv * c.hd / 16, per_head = c.hd / 16;
+    const bool is_v = blockIdx.y;
+    const int64_t total = n_tok * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t t = i / pieces;
+        const int p = (int)(i - t * pieces), head = p / per_head, e = p - head * per_head;
+        const int64_t s = slot[t], pg = s >> c.page_shift;
+        T *dst = (is_v ? v : k) + (t * c.hkv + head) * c.hd + e * 16;
+        if (s < 0 || pg >= c.n_pages) {
+            if (s >= 0) atomicOr(status, STATUS_BAD_PLAN);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) store4(dst + 4 * j, 0.0f, 0.0f, 0.0f, 0.0f);
+            continue;
+        }
+        const int64_t blk = kv8_block(c, (int)pg, head, (int)(s & (c.page - 1)) >> 4);
+        const float sc = (is_v ? c.vs : c.ks)[blk];
+        const int8_t *src = (is_v ? c.v : c.k) + (blk * KV8_BLOCK + (s & (KV8_BLOCK - 1))) * c.hd + e * 16;
+        const uint4 w = *reinterpret_cast<const uint4 *>(src);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            store4(dst + 4 * j, (float)(int8_t)u[j] * sc, (float)(int8_t)(u[j] >> 8) * sc,
+                   (float)(int8_t)(u[j] >> 16) * sc, (float)(int8_t)(u[j] >> 24) * sc);
+    }
+}
+
+template <typename T>
+int store_typed(const Kv8Dev &c, const void *k, const void *v, int64_t k_stride, int64_t v_stride, const int64_t *slot,
+                const int32_t *pos, const RopeDev &rope, int64_t n_tok, int num_sms, int *status, cudaStream_t st) {
+    // Tokens per CTA: as many as keep two CTAs per SM busy, so that a prompt's
+    // CTAs (one or two runs per 16 tokens) are few and a decode batch's runs
+    // (one per token) spread over the GPU.
+    int chunk = 32;
+    while (chunk > 2 && (n_tok + chunk - 1) / chunk * c.hkv < 2 * num_sms) chunk >>= 1;
+    const dim3 grid((unsigned)((n_tok + chunk - 1) / chunk), (unsigned)c.hkv);
+    const T *kt = static_cast<const T *>(k), *vt = static_cast<const T *>(v);
+    switch (c.hd) {
+        case 64:
+            kv8_store_kernel<T, 64><<<grid, STORE_WARPS * 32, 0, st>>>(c, kt, vt, k_stride, v_stride, slot, pos, rope, n_tok, chunk, status);
+            break;
+        case 96:
+            kv8_store_kernel<T, 96><<<grid, STORE_WARPS * 32, 0, st>>>(c, kt, vt, k_stride, v_stride, slot, pos, rope, n_tok, chunk, status);
+            break;
+        case 128:
+            kv8_store_kernel<T, 128><<<grid, STORE_WARPS * 32, 0, st>>>(c, kt, vt, k_stride, v_stride, slot, pos, rope, n_tok, chunk, status);
+            break;
+        case 256:
+            kv8_store_kernel<T, 256><<<grid, STORE_WARPS * 32, 0, st>>>(c, kt, vt, k_stride, v_stride, slot, pos, rope, n_tok, chunk, status);
+            break;
+        default: return -3;
+    }
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace
+
+int launch_kv8_plan(const Kv8PlanLaunch &L, cudaStream_t st) {
+    // One CTA while a step has few tokens (decode: a cluster's launch and
+    // barrier cost more than they share out), eight for steps with prompts.
+    const int ctas = L.max_tok > 4 * PLAN_THREADS ? 8 : 1;
+    const size_t smem = (size_t)(3 * L.n_seq + 2) * 4;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kv8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return -2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv8_plan_kernel, L) == cudaSuccess ? 0 : -2;
+}
+
+int launch_kv8_release(const int32_t *drop, int32_t *len, int n_seq, int page_shift, const int32_t *table,
+                       int64_t max_pages, int32_t *free_pages, int64_t n_pages, int32_t *n_free, int *status,
+                       cudaStream_t st) {
+    kv8_release_kernel<<<1, PLAN_THREADS, (size_t)(n_seq + 1) * 4, st>>>(drop, len, n_seq, page_shift, table, max_pages,
+                                                                       free_pages, n_pages, n_free, status);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+int launch_kv8_store(const Kv8Dev &c, bool f16, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
+                     const int64_t *slot, const int32_t *pos, const RopeDev &rope, int64_t n_tok, int num_sms,
+                     int *status, cudaStream_t st) {
+    return f16 ? store_typed<__half>(c, k, v, k_stride, v_stride, slot, pos, rope, n_tok, num_sms, status, st)
+               : store_typed<float>(c, k, v, k_stride, v_stride, slot, pos, rope, n_tok, num_sms, status, st);
+}
+
+int launch_kv8_load(const Kv8Dev &c, bool f16, const int64_t *slot, int64_t n_tok, void *k, void *v, int *status,
+                    cudaStream_t st) {
+    const int64_t items = n_tok * (c.hkv * c.hd / 16);
+    const int64_t ctas = (items + 255) / 256;
+    const dim3 grid((unsigned)(ctas < (1 << 20) ? ctas : (1 << 20)), 2);
+    if (f16)
+        kv8_load_kernel<__half><<<grid, 256, 0, st>>>(c, slot, n_tok, static_cast<__half *>(k), static_cast<__half *>(v), status);
+    else
+        kv8_load_kernel<float><<<grid, 256, 0, st>>>(c, slot, n_tok, static_cast<float *>(k), static_cast<float *>(v), status);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace sicu

@@ -1,0 +1,116 @@
+// The paged 8-bit KV cache as the kernels see it: addressing, RoPE of a
+// token's rows at its own position, and the launch parameters shared by the
+// store and attention kernels. Layout and semantics: include/siphon_cuda.h.
+#pragma once
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace sicu {
+
+// Block id within a KV head of the cache: page * hkv + head selects the
+// head's page, sub the 16-token block inside it. The same index addresses the
+// block's scale and, times 16 * hd, its codes (64-bit: a cache passes 2^31
+// codes at a quarter of a million tokens of 8 heads of 128 channels, K alone).
+__device__ __forceinline__ int64_t kv8_block(const Kv8Dev &c, int page, int head, int sub) {
+    return ((int64_t)page * c.hkv + head) * (c.page / KV8_BLOCK) + sub;
+}
+
+// Eight channels of one row: neox pairs (j, j + hd/2) live in a and b at the
+// same index, adjacent pairs inside a and inside b. Both forms use table
+// entries 4 c .. 4 c + 3 of the position's row.
+struct Oct {
+    float a[4], b[4];
+};
+__device__ __forceinline__ int oct_a(int c, int neox) { return neox ? 4 * c : 8 * c; }
+__device__ __forceinline__ int oct_b(int c, int hd, int neox) { return neox ? hd / 2 + 4 * c : 8 * c + 4; }
+
+// x0' = x0 c - x1 s, x1' = x0 s + x1 c with each product rounded on its own
+// (no contraction), so the result does not depend on how a caller's own f32
+// code is compiled.
+__device__ __forceinline__ void rot(float &x0, float &x1, float c, float s) {
+    const float a = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
+    x1 = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
+    x0 = a;
+}
+__device__ __forceinline__ void rope_oct(Oct &o, const RopeDev &r, int64_t pos, int c) {
+    if (4 * c >= r.half) return;                    // channels from n_rot on stay as they are
+    const float4 cs = __ldg(reinterpret_cast<const float4 *>(r.cs + pos * r.half + 4 * c));
+    const float4 sn = __ldg(reinterpret_cast<const float4 *>(r.sn + pos * r.half + 4 * c));
+    if (r.neox) {
+        rot(o.a[0], o.b[0], cs.x, sn.x);
+        rot(o.a[1], o.b[1], cs.y, sn.y);
+        rot(o.a[2], o.b[2], cs.z, sn.z);
+        rot(o.a[3], o.b[3], cs.w, sn.w);
+    } else {
+        rot(o.a[0], o.a[1], cs.x, sn.x);
+        rot(o.a[2], o.a[3], cs.y, sn.y);
+        rot(o.b[0], o.b[1], cs.z, sn.z);
+        rot(o.b[2], o.b[3], cs.w, sn.w);
+    }
+}
+
+// four consecutive values as f32
+__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+    const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void load4(const __half *p, float (&v)[4]) {
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+    v[0] = h2f(x.x & 0xffffu); v[1] = h2f(x.x >> 16); v[2] = h2f(x.y & 0xffffu); v[3] = h2f(x.y >> 16);
+}
+__device__ __forceinline__ void store4(float *p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void store4(__half *p, float a, float b, float c, float d) {
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t *>(&x);
+    u.y = *reinterpret_cast<const uint32_t *>(&y);
+    *reinterpret_cast<uint2 *>(p) = u;
+}
+__device__ __forceinline__ void store1(float *p, float a) { *p = a; }
+__device__ __forceinline__ void store1(__half *p, float a) { *p = __float2half_rn(a); }
+
+// A request of the batch, its device-resident numbers brought inside the
+// bounds the host was given (anything outside sets STATUS_BAD_PLAN): rows
+// [t0, t0 + n_new) of the packed tensors at positions len - n_new ...
+struct Kv8Seq {
+    int t0, n_new, len, prefix, first;
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnDev &a, int i) {
+    Kv8Seq s;
+    const int c0 = __ldg(a.cu + i), c1 = __ldg(a.cu + i + 1), len = __ldg(a.len + i);
+    s.prefix = a.prefix ? __ldg(a.prefix + i) : 0;
+    s.first = a.first ? __ldg(a.first + i) : 0;
+    const bool bad = c0 < 0 || c1 < c0 || c1 > a.n_tok || len < 0 || len > a.max_len || c1 - c0 > a.max_new ||
+                     c1 - c0 > len;
+    if (bad) {
+        atomicOr(a.status, STATUS_BAD_PLAN);
+        s.t0 = s.n_new = s.len = 0;
+        return s;
+    }
+    s.t0 = c0;
+    s.n_new = c1 - c0;
+    s.len = len;
+    if (s.prefix > len) s.prefix = len;
+    if (s.first < 0) s.first = 0;
+    return s;
+}
+// positions row p sees: [lo, hi), empty when lo >= hi
+__device__ __forceinline__ int kv8_lo(const Kv8AttnDev &a, const Kv8Seq &s, int p) {
+    const int w = a.window > 0 ? p + 1 - a.window : 0;
+    return w > s.first ? w : s.first;
+}
+__device__ __forceinline__ int kv8_hi(const Kv8Seq &s, int p) { return p + 1 > s.prefix ? p + 1 : s.prefix; }
+
+// page of token block b (16 tokens) of request i; an id outside the pool sets
+// STATUS_BAD_PLAN and reads page 0 instead
+__device__ __forceinline__ int kv8_page(const Kv8Dev &c, const Kv8AttnDev &a, int i, int b) {
+    const int p = __ldg(a.table + (int64_t)i * a.max_pages + (b >> (c.page_shift - 4)));
+    if ((unsigned)p < (unsigned)c.n_pages) return p;
+    atomicOr(a.status, STATUS_BAD_PLAN);
+    return 0;
+}
+
+}  // namespace sicu

@@ -1,0 +1,523 @@
+// Attention over the paged 8-bit KV cache: the kernel for single tokens and
+// short rows (mma.sync, keys split over CTAs) and its combine.
+//
+//   z_rj = log2(e) * f(scale * q_r . k_j),  f = the cap and the distance bias
+//   out_r = sum_j 2^(z_rj - m_r) v_j / sum_j 2^(z_rj - m_r)   over visible j
+//
+// The rows of one KV head (its n_head / n_head_kv query heads times a
+// request's new tokens) are the N side of m16n8k16 products, the cache the M
+// side: a warp takes 16 keys (one quantization block: one scale each for K
+// and V), loads their K and V codes straight into registers in an order of
+// channels and keys that makes every register an operand fragment after
+// byte -> f16 expansion (|code| <= 127 is exact in f16), forms S^T = K Q^T,
+// the weights in f32, and accumulates O^T += V^T P^T. Sums, maxima and the
+// output stay in f32.
+//
+// The rotated q enters as two f16 parts (hi + lo, 22 bits), so scores agree
+// with an f32 computation. So do f32 callers' weights; f16 callers' weights
+// are rounded once to f16 (2^-11, the size of the output's own rounding).
+#include "kv8.cuh"
+#include "tc.cuh"
+
+namespace sicu {
+namespace {
+
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr int AT_WARPS = 4;
+// A new maximum rescales the accumulator only when it passes the running one
+// by 2^8: weights stay below 2^8 and f16 carries them as precisely.
+constexpr float AT_LAZY = 8.0f;
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+// two codes biased by 128 (bytes i, j of x) as exact halves: 0x6400 | u is 1024 + u
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t sel) {
+    const uint32_t h = prmt(x, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __floats2half2_rn(1152.0f, 1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// cap * tanh(x / cap) as cap - 2 cap / (1 + e^(2 x / cap)): absolute error a
+// few 2^-23 of the cap, saturating without overflow
+__device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
+    const float e = ex2(x * inv_cap * (2.0f * LOG2E));
+    return cap - 2.0f * cap * __fdividef(1.0f, 1.0f + fminf(e, 1e30f));
+}
+
+// weight of a part with maximum mp under the joint maximum m: parts that saw
+// no key (both -inf) keep their zero sums, and a NaN sum stays NaN
+__device__ __forceinline__ float join(float mp, float m) { return mp == m ? 1.0f : ex2(mp - m); }
+// 1 / l; a row that sees no key (l = 0) is zero
+__device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l); }
+
+template <int W>
+__device__ __forceinline__ void ldg_words(const int8_t *p, uint32_t *w) {
+    if constexpr (W == 4) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else if constexpr (W == 2) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = x.x; w[1] = x.y;
+    } else {
+        w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    }
+}
+
+struct AttnGeom {
+    int splits;        // CTAs a request's keys may be dealt to
+    int chunk;         // keys per CTA (a multiple of 16)
+    int row_tiles;     // row tiles per KV head
+    int rows;          // rows kept per tile in the workspace
+};
+
+// Partial results of one (request, KV head, row tile, split): rows x hd f32,
+// then (m, l) per row, padded to 16 bytes (the next part is written in float4s).
+__host__ __device__ inline int64_t part_floats(int rows, int hd) { return ((int64_t)rows * (hd + 2) + 3) & ~(int64_t)3; }
+__device__ __forceinline__ int64_t part_index(const AttnGeom &g, int hkv, int seq, int head, int rt, int split) {
+    return (((int64_t)seq * hkv + head) * g.row_tiles + rt) * g.splits + split;
+}
+
+// visible key range of a row tile, start rounded down to a block
+struct Span {
+    int b0, b1;        // blocks [b0, b1)
+};
+__device__ __forceinline__ Span tile_span(const Kv8AttnDev &a, const Kv8Seq &s, int t_lo, int t_hi) {
+    const int p0 = s.len - s.n_new + t_lo, p1 = s.len - s.n_new + t_hi;
+    const int lo = kv8_lo(a, s, p0), hi = kv8_hi(s, p1);
+    Span r;
+    r.b0 = lo >> 4;
+    r.b1 = lo < hi ? (hi + 15) >> 4 : r.b0;
+    return r;
+}
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int R = 8 * NT, KW = HD / 16, VW = HD / 32, WPC = HD % 64 == 0 ? 4 : 2;
+    constexpr int VL = HD % 128 == 0 ? 4 : HD % 64 == 0 ? 2 : 1;
+    constexpr int PARTS = SPLIT ? 2 : 1;        // of the weights
+    // q fragments: [word][n tile][hi, lo][lane] pairs of f16x2
+    __shared__ __align__(16) uint2 qf[KW * NT * 2 * 32];
+    __shared__ __align__(16) float qrow[R * HD];       // rotated q; the merged output later
+    __shared__ float rscale[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
+    __shared__ int row_lo[R], row_hi[R], row_pos[R];
+    __shared__ float row_slope[R];
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
+    const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, split = blockIdx.y, seq = blockIdx.z;
+    const Kv8Seq s = kv8_seq(a, seq);
+    const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
+    if (rt * R >= n_rows) return;
+    const int rows = min(R, n_rows - rt * R);
+    const Span sp = tile_span(a, s, rt * R / group, (rt * R + rows - 1) / group);
+    const int cb = g.chunk >> 4;
+    const int parts = (sp.b1 - sp.b0 + cb - 1) / cb;
+    if (split >= max(parts, 1)) return;
+
+    // ---- q: rows rotated at their positions, scaled by a power of two, as fragments
+    const T *q = static_cast<const T *>(a.q);
+    for (int i = tid; i < R * (HD / 8); i += AT_WARPS * 32) {
+        const int r = i / (HD / 8), o = i % (HD / 8), rr = rt * R + r, neox = a.rope.neox;
+        Oct x;
+        if (r < rows) {
+            const int t = rr / group, h = head * group + rr % group;
+            const T *src = q + (int64_t)(s.t0 + t) * a.q_stride + (int64_t)h * HD;
+            load4(src + oct_a(o, neox), x.a);
+            load4(src + oct_b(o, HD, neox), x.b);
+            if (a.rope.half) {
+                const int64_t p = s.len - s.n_new + t;
+                if (p < a.rope.rows) rope_oct(x, a.rope, p, o);
+                else if (o == 0) atomicOr(a.status, STATUS_BAD_PLAN);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.a[e] = x.b[e] = 0.0f;
+        }
+        store4(qrow + r * HD + oct_a(o, neox), x.a[0], x.a[1], x.a[2], x.a[3]);
+        store4(qrow + r * HD + oct_b(o, HD, neox), x.b[0], x.b[1], x.b[2], x.b[3]);
+    }
+    __syncthreads();
+    // A row's largest magnitude is brought to [1, 2) by a power of two, so
+    // that its f16 parts neither overflow nor lose small rows; the factor
+    // goes back in with the score's scale.
+    for (int r = warp; r < R; r += AT_WARPS) {
+        float m = 0.0f;
+        for (int d = lane; d < HD; d += 32) m = fmaxf(m, fabsf(qrow[r * HD + d]));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if (lane == 0) {
+            // exponent of the magnitude, kept where both factors are normal
+            const int e = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
+            rscale[r] = __uint_as_float((uint32_t)(127 + e) << 23);
+            if (r < rows) {
+                const int t = (rt * R + r) / group, p = s.len - s.n_new + t;
+                row_pos[r] = p;
+                row_lo[r] = kv8_lo(a, s, p);
+                row_hi[r] = kv8_hi(s, p);
+                row_slope[r] = a.slopes ? __ldg(a.slopes + head * group + (rt * R + r) % group) * LOG2E : 0.0f;
+            } else {
+                row_pos[r] = row_lo[r] = row_hi[r] = 0;
+                row_slope[r] = 0.0f;
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < KW * NT * 32; i += AT_WARPS * 32) {
+        const int ln = i & 31, nt = (i >> 5) % NT, w = i / (32 * NT);
+        const int r = nt * 8 + (ln >> 2), d = (w / WPC) * (16 * WPC) + (ln & 3) * (4 * WPC) + (w % WPC) * 4;
+        const float inv = __fdiv_rn(1.0f, rscale[r]);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = qrow[r * HD + d + e] * inv;
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = x[e] - __half2float(__float2half_rn(x[e]));
+        qf[((w * NT + nt) * 2) * 32 + ln] = make_uint2(half2_bits(x[0], x[1]), half2_bits(x[2], x[3]));
+        qf[((w * NT + nt) * 2 + 1) * 32 + ln] = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
+    }
+    __syncthreads();
+
+    // ---- keys
+    // per thread: two rows (columns of the C fragment) per n tile
+    float mrun[NT][2], lsum[NT][2], rs[NT][2];
+    float o[HD / 16][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mrun[nt][e] = -INFINITY;
+            lsum[nt][e] = 0.0f;
+            rs[nt][e] = rscale[nt * 8 + 2 * tq + e] * a.scale;
+        }
+#pragma unroll
+    for (int mt = 0; mt < HD / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
+    float vref = 0.0f;                   // the V scale the accumulator is in units of
+    // the keys every row of the tile sees need no mask
+    int all_lo = 0, all_hi = INT_MAX;
+    for (int r = 0; r < rows; ++r) {
+        all_lo = max(all_lo, row_lo[r]);
+        all_hi = min(all_hi, row_hi[r]);
+    }
+    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const int blk_end = min(sp.b1, sp.b0 + (split + 1) * cb);
+    uint32_t kw[2][KW], vw[4][VW];
+    float ks = 0.0f, vs = 0.0f;
+    auto load = [&](int b) {
+        const int pg = kv8_page(c, a, seq, b);
+        const int64_t blk = kv8_block(c, pg, head, b & (c.page / KV8_BLOCK - 1));
+        ks = __ldg(c.ks + blk);
+        vs = __ldg(c.vs + blk);
+        const int8_t *kb = c.k + blk * (KV8_BLOCK * HD), *vb = c.v + blk * (KV8_BLOCK * HD);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int w = 0; w < KW; w += WPC)
+                ldg_words<WPC>(kb + (gq + 8 * r) * HD + (w / WPC) * (16 * WPC) + tq * (4 * WPC), &kw[r][w]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < VW; w += VL)
+                ldg_words<VL>(vb + (2 * tq + (r & 1) + 8 * (r >> 1)) * HD + gq * (HD / 8) + w * 4, &vw[r][w]);
+    };
+    int b = sp.b0 + split * cb + warp;
+    if (b < blk_end) load(b);
+    for (; b < blk_end; b += AT_WARPS) {
+        // S^T: 16 keys x R rows
+        float z[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[nt][e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const uint32_t x = kw[0][w] ^ 0x80808080u, y = kw[1][w] ^ 0x80808080u;
+            const uint32_t af[4] = {code_pair(x, 0x4140), code_pair(y, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4342)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint2 f = qf[((w * NT + nt) * 2 + p) * 32 + lane];
+                    mma_f16(z[nt], af, f.x, f.y);
+                }
+        }
+        const float kscale = ks, vscale = vs;
+        uint32_t vcur[4][VW];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vcur[r][w] = vw[r][w] ^ 0x80808080u;
+        const int j0 = b * KV8_BLOCK + gq;           // this thread's keys: j0 and j0 + 8
+        if (b + AT_WARPS < blk_end) load(b + AT_WARPS);
+        const bool masked = (b << 4) < all_lo || (b << 4) + 16 > all_hi;
+        bool grow = vscale > vref;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
+                float x = z[nt][e] * (rs[nt][e & 1] * kscale);
+                if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
+                x *= LOG2E;
+                if (a.slopes) x -= row_slope[r] * fabsf((float)(row_pos[r] - j));
+                if (masked && (j < row_lo[r] || j >= row_hi[r])) x = -INFINITY;
+                z[nt][e] = x;
+                grow |= x > mrun[nt][e & 1] + AT_LAZY;
+            }
+        if (__any_sync(0xffffffffu, grow)) {
+            // new maxima (over the 16 keys: lanes with the same tq) and V unit
+            const float vnew = fmaxf(vref, vscale), vf = vnew > 0.0f ? __fdividef(vref, vnew) : 0.0f;
+            vref = vnew;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(z[nt][e], z[nt][e + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+                    m = fmaxf(m, mrun[nt][e]);
+                    const float f = m == -INFINITY ? 1.0f : ex2(mrun[nt][e] - m);
+                    mrun[nt][e] = m;
+                    lsum[nt][e] *= f;
+#pragma unroll
+                    for (int mt = 0; mt < HD / 16; ++mt) {
+                        o[mt][nt][e] *= f * vf;
+                        o[mt][nt][e + 2] *= f * vf;
+                    }
+                }
+        }
+        // weights, in units of the running V scale for the second product
+        const float vr = vref > 0.0f ? __fdividef(vscale, vref) : 0.0f;
+        uint32_t pf[NT][PARTS][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float m = mrun[nt][e & 1];
+                const float p = ex2(z[nt][e] - (m == -INFINITY ? 0.0f : m));
+                lsum[nt][e & 1] += p;
+                w[e] = p * vr;
+            }
+            pf[nt][0][0] = movm_t(half2_bits(w[0], w[1]));
+            pf[nt][0][1] = movm_t(half2_bits(w[2], w[3]));
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] -= __half2float(__float2half_rn(w[e]));
+                pf[nt][1][0] = movm_t(half2_bits(w[0], w[1]));
+                pf[nt][1][1] = movm_t(half2_bits(w[2], w[3]));
+            }
+        }
+        // O^T += V^T P^T: a word holds four channels, two per m tile
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            const uint32_t x0 = prmt(vcur[0][w], vcur[1][w], 0x5140), x1 = prmt(vcur[0][w], vcur[1][w], 0x7362);
+            const uint32_t y0 = prmt(vcur[2][w], vcur[3][w], 0x5140), y1 = prmt(vcur[2][w], vcur[3][w], 0x7362);
+            const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
+            const uint32_t hi[4] = {code_pair(x1, 0x4140), code_pair(x1, 0x4342), code_pair(y1, 0x4140), code_pair(y1, 0x4342)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    mma_f16(o[2 * w][nt], lo, pf[nt][p][0], pf[nt][p][1]);
+                    mma_f16(o[2 * w + 1][nt], hi, pf[nt][p][0], pf[nt][p][1]);
+                }
+        }
+    }
+
+    // ---- the four warps' parts, then this CTA's
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float l = lsum[nt][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+            if (gq == 0) {
+                sm_m[warp][nt * 8 + 2 * tq + e] = mrun[nt][e];
+                sm_l[warp][nt * 8 + 2 * tq + e] = l;
+            }
+        }
+    if (lane == 0) sm_vr[warp] = vref;
+    __syncthreads();
+    float f[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = nt * 8 + 2 * tq + e;
+            float m = sm_m[0][r];
+            for (int w = 1; w < AT_WARPS; ++w) m = fmaxf(m, sm_m[w][r]);
+            f[nt][e] = join(sm_m[warp][r], m) * sm_vr[warp];
+        }
+    for (int w = 0; w < AT_WARPS; ++w) {
+        if (warp == w) {
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = nt * 8 + 2 * tq + (e & 1), d = gq * (HD / 8) + 2 * mt + (e >> 1);
+                        const float x = o[mt][nt][e] * f[nt][e & 1];
+                        if (w == 0) qrow[r * HD + d] = x;
+                        else qrow[r * HD + d] += x;
+                    }
+        }
+        __syncthreads();
+    }
+    float *part_o = ws, *part_ml = nullptr;
+    if (parts > 1) {
+        const int64_t pi = part_index(g, c.hkv, seq, head, rt, split);
+        part_o = ws + pi * part_floats(g.rows, HD);
+        part_ml = part_o + (int64_t)g.rows * HD;
+    }
+    for (int i = tid; i < rows * (HD / 4); i += AT_WARPS * 32) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        float m = sm_m[0][r], l = 0.0f;
+        for (int w = 1; w < AT_WARPS; ++w) m = fmaxf(m, sm_m[w][r]);
+        for (int w = 0; w < AT_WARPS; ++w) l += sm_l[w][r] * join(sm_m[w][r], m);
+        const float4 x = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
+        if (parts > 1) {
+            *reinterpret_cast<float4 *>(part_o + r * HD + d) = x;
+            if (d == 0) {
+                part_ml[2 * r] = m;
+                part_ml[2 * r + 1] = l;
+            }
+        } else {
+            const float inv = inv_sum(l);
+            const int rr = rt * R + r, t = rr / group, h = head * group + rr % group;
+            store4(static_cast<T *>(a.out) + (int64_t)(s.t0 + t) * a.out_stride + (int64_t)h * HD + d, x.x * inv, x.y * inv,
+                   x.z * inv, x.w * inv);
+        }
+    }
+}
+
+// Joins the splits of a row in split order: one warp per row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, int R, const float *ws) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, seq = blockIdx.z;
+    const Kv8Seq s = kv8_seq(a, seq);
+    const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
+    if (rt * R >= n_rows) return;
+    const int rows = min(R, n_rows - rt * R), r = blockIdx.y * 4 + warp;
+    const Span sp = tile_span(a, s, rt * R / group, (rt * R + rows - 1) / group);
+    const int cb = g.chunk >> 4, parts = (sp.b1 - sp.b0 + cb - 1) / cb;
+    if (parts <= 1 || r >= rows) return;
+    const int64_t stride = part_floats(g.rows, HD);
+    const float *p0 = ws + part_index(g, c.hkv, seq, head, rt, 0) * stride;
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p0[i * stride + g.rows * HD + 2 * r]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float l = 0.0f, acc[HD / 32];
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.0f;
+    for (int i = 0; i < parts; ++i) {
+        const float *p = p0 + i * stride;
+        const float f = join(p[g.rows * HD + 2 * r], m);
+        l += p[g.rows * HD + 2 * r + 1] * f;
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) acc[e] += p[r * HD + e * 32 + lane] * f;
+    }
+    const float inv = inv_sum(l);
+    const int rr = rt * R + r, t = rr / group, h = head * group + rr % group;
+    T *out = static_cast<T *>(a.out) + (int64_t)(s.t0 + t) * a.out_stride + (int64_t)h * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) store1(out + e * 32 + lane, acc[e] * inv);
+}
+
+// n tiles per CTA: the rows of a request's longest piece, up to 32 (16 with
+// 256 channels, whose accumulator would not fit the registers)
+int attn_nt(const Kv8Dev &c, const Kv8AttnDev &a) {
+    const int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
+    return rows <= 8 ? 1 : rows <= 16 || c.hd == 256 ? 2 : 4;
+}
+
+AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
+    const int nt = attn_nt(c, a), R = 8 * nt;
+    const int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
+    AttnGeom g;
+    g.row_tiles = (int)((rows + R - 1) / R);
+    g.rows = (int)(rows < R ? rows : R);
+    // Keys per CTA: enough CTAs for four per SM and two rounds of them, each
+    // with at least 256 keys.
+    const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, want = 8 * (int64_t)num_sms;
+    int64_t splits = (want + units - 1) / units;
+    int64_t chunk = (a.max_len + splits - 1) / splits;
+    if (chunk < 256) chunk = 256;
+    chunk = (chunk + 63) / 64 * 64;
+    g.chunk = (int)chunk;
+    // a span rounded down to a block may begin 15 keys early
+    g.splits = (int)((a.max_len + 15 + chunk - 1) / chunk);
+    return g;
+}
+
+template <typename T, int HD, int NT>
+int launch_typed(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
+    const dim3 grid((unsigned)(g.row_tiles * c.hkv), (unsigned)g.splits, (unsigned)a.n_seq);
+    kv8_attn_kernel<T, HD, NT><<<grid, AT_WARPS * 32, 0, st>>>(c, a, g, ws);
+    if (cudaGetLastError() != cudaSuccess) return -2;
+    if (g.splits > 1) {
+        const dim3 cgrid((unsigned)(g.row_tiles * c.hkv), (unsigned)((g.rows + 3) / 4), (unsigned)a.n_seq);
+        kv8_combine_kernel<T, HD><<<cgrid, 128, 0, st>>>(c, a, g, 8 * NT, ws);
+        if (cudaGetLastError() != cudaSuccess) return -2;
+    }
+    return 0;
+}
+
+template <typename T, int HD>
+int launch_hd(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
+    switch (attn_nt(c, a)) {
+        case 1: return launch_typed<T, HD, 1>(c, a, g, ws, st);
+        case 2: return launch_typed<T, HD, 2>(c, a, g, ws, st);
+        default:
+            if constexpr (HD <= 128) return launch_typed<T, HD, 4>(c, a, g, ws, st);
+            return -3;
+    }
+}
+
+template <typename T>
+int launch_t(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
+    switch (c.hd) {
+        case 64: return launch_hd<T, 64>(c, a, g, ws, st);
+        case 96: return launch_hd<T, 96>(c, a, g, ws, st);
+        case 128: return launch_hd<T, 128>(c, a, g, ws, st);
+        case 256: return launch_hd<T, 256>(c, a, g, ws, st);
+        default: return -3;
+    }
+}
+
+}  // namespace
+
+size_t kv8_attn_workspace(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int num_sms) {
+    (void)f16;
+    const AttnGeom g = attn_geom(c, a, num_sms);
+    if (g.splits <= 1) return 0;
+    return (size_t)a.n_seq * c.hkv * g.row_tiles * g.splits * part_floats(g.rows, c.hd) * 4;
+}
+
+int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *ws, int num_sms, cudaStream_t st) {
+    const AttnGeom g = attn_geom(c, a, num_sms);
+    return f16 ? launch_t<__half>(c, a, g, static_cast<float *>(ws), st)
+               : launch_t<float>(c, a, g, static_cast<float *>(ws), st);
+}
+
+}  // namespace sicu

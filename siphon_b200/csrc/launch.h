@@ -208,4 +208,62 @@ int launch_dequant(uint32_t wtype, const void *w, int64_t n_in, const int64_t *r
 // greedy choice (first maximum) of m rows of n floats into out[m]
 int launch_argmax(const float *x, int64_t n, int64_t m, int64_t *out, cudaStream_t st);
 
+// ---- paged 8-bit KV cache (kv8.cu, kv8_attn.cu) ----
+constexpr int KV8_BLOCK = 16;         // tokens that share a scale
+constexpr int KV8_MAX_SEQ = 8192;     // requests per step
+struct Kv8Dev {
+    int8_t *k, *v;                    // [n_pages][hkv][page][hd]
+    float *ks, *vs;                   // [n_pages][hkv][page / 16]
+    int64_t n_pages;
+    int page, page_shift, hkv, hd;
+};
+struct RopeDev {
+    const float *cs = nullptr, *sn = nullptr;   // [rows][half]
+    int64_t rows = 0;
+    int half = 0;                     // n_rot / 2; 0: no rotation
+    int neox = 0;
+};
+struct Kv8PlanLaunch {
+    const int32_t *past, *fresh;
+    int n_seq, page_shift, max_pages;
+    int32_t *table;
+    const int32_t *free_pages;
+    int64_t n_pages;
+    const int32_t *n_free;
+    int32_t *n_free_out;
+    int64_t max_tok;
+    int32_t *cu, *len;
+    int64_t *slot;
+    int32_t *pos;
+    int *status;
+};
+int launch_kv8_plan(const Kv8PlanLaunch &L, cudaStream_t st);
+int launch_kv8_release(const int32_t *drop, int32_t *len, int n_seq, int page_shift, const int32_t *table,
+                       int64_t max_pages, int32_t *free_pages, int64_t n_pages, int32_t *n_free, int *status,
+                       cudaStream_t st);
+// f16: k and v hold halves instead of floats
+int launch_kv8_store(const Kv8Dev &c, bool f16, const void *k, const void *v, int64_t k_stride, int64_t v_stride,
+                     const int64_t *slot, const int32_t *pos, const RopeDev &rope, int64_t n_tok, int num_sms,
+                     int *status, cudaStream_t st);
+int launch_kv8_load(const Kv8Dev &c, bool f16, const int64_t *slot, int64_t n_tok, void *k, void *v, int *status,
+                    cudaStream_t st);
+struct Kv8AttnDev {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;     // elements between tokens
+    int n_tok, n_head, n_seq;
+    const int32_t *table, *len, *cu;
+    int64_t max_pages;
+    int max_new, max_len;
+    float scale, cap;
+    const float *slopes;
+    int window;
+    const int32_t *prefix, *first;
+    RopeDev rope;
+    int *status;
+};
+// workspace of an attention call (a bound over every batch of these sizes)
+size_t kv8_attn_workspace(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int num_sms);
+int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *ws, int num_sms, cudaStream_t st);
+
 }  // namespace sicu

@@ -83,6 +83,12 @@ SIGNATURES = {
                             C.c_float, _fp, _vp],
     "sicu_attention_prompt": [_fp, _fp, _fp, _vp, _vp, _fp, _fp, _i64, _i64, _i64, _i64, C.c_int, _i64, _i64,
                               _i64, C.c_float, _fp, _vp],
+    "sicu_kv8_plan": [_vp, _vp, _i64, C.c_int32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp],
+    "sicu_kv8_release": [_vp, _vp, _i64, C.c_int32, _vp, _i64, _vp, _i64, _vp, _vp],
+    "sicu_kv8_store": [_vp, _u32, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
+    "sicu_kv8_load": [_vp, _u32, _vp, _i64, _vp, _vp, _vp],
+    "sicu_kv8_attention_ws": [_vp, _vp, C.POINTER(C.c_size_t)],
+    "sicu_kv8_attention": [_vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp],
 }
 
 PRO_NONE, PRO_RMS_NORM, PRO_SWIGLU, PRO_MUL = 0, 1, 2, 3
@@ -99,6 +105,8 @@ class Prologue(C.Structure):
 TC_F16, TC_I8 = 0, 1       # sicu_tc_peak kinds
 AR_HANDLE_BYTES = 64
 STATUS_WAIT_TIMEOUT, STATUS_AR_TIMEOUT, STATUS_BAD_ROW = 1, 2, 4
+STATUS_NO_PAGES, STATUS_BAD_PLAN, STATUS_NONFINITE = 8, 16, 32
+T_F32, T_F16 = 0, 1        # activation types of the sicu_kv8_* entry points
 
 
 def rms_norm_step(weight, eps: float, residual=None, sum_out=None) -> Prologue:
@@ -114,6 +122,47 @@ def swiglu_step(up) -> Prologue:
 def mul_step(up) -> Prologue:
     """a = x * up (x already through silu: the gate product's EPI_SILU)."""
     return Prologue(PRO_MUL, 0.0, None, None, None, _ptr(up))
+
+
+class Kv8(C.Structure):
+    """sicu_kv8: one layer's paged 8-bit KV cache (the arrays must outlive it)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int64), ("page", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class RopeTables(C.Structure):
+    """sicu_rope_tables: cos / sin by position."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("rows", C.c_int64), ("n_rot", C.c_int32),
+                ("neox", C.c_int32)]
+
+
+class Kv8Attn(C.Structure):
+    """sicu_kv8_attn: what an attention call over the paged cache is given."""
+    _fields_ = [("type", C.c_uint32), ("n_head", C.c_int32), ("n_tok", C.c_int64), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("table", C.c_void_p), ("max_pages", C.c_int64), ("len", C.c_void_p),
+                ("cu", C.c_void_p), ("n_seq", C.c_int64), ("max_new", C.c_int64), ("max_len", C.c_int64),
+                ("scale", C.c_float), ("cap", C.c_float), ("slopes", C.c_void_p), ("window", C.c_int64),
+                ("prefix", C.c_void_p), ("first", C.c_void_p), ("rope", C.POINTER(RopeTables))]
+
+
+def kv8_cache(k, v, k_scale, v_scale, n_pages: int, page: int, n_head_kv: int, head_dim: int) -> Kv8:
+    """k, v: int8 [n_pages][n_head_kv][page][head_dim]; k_scale, v_scale: f32
+    [n_pages][n_head_kv][page / 16]."""
+    return Kv8(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), n_pages, page, n_head_kv, head_dim)
+
+
+def rope(cos, sin, rows: int, n_rot: int, neox: bool = False) -> RopeTables:
+    """cos / sin tables [rows][n_rot / 2] of positions 0 .. rows - 1."""
+    return RopeTables(_ptr(cos), _ptr(sin), rows, n_rot, 1 if neox else 0)
+
+
+def kv8_attn(type: int, n_head: int, n_tok: int, table, max_pages: int, length, cu, n_seq: int, max_new: int,
+             max_len: int, scale: float, cap: float = 0.0, slopes=None, window: int = 0, prefix=None, first=None,
+             rope: RopeTables | None = None, q_stride: int = 0, out_stride: int = 0) -> Kv8Attn:
+    """The description of a step's attention (arrays and tables must outlive it)."""
+    return Kv8Attn(type, n_head, n_tok, q_stride, out_stride, _ptr(table), max_pages, _ptr(length), _ptr(cu), n_seq,
+                   max_new, max_len, scale, cap, _ptr(slopes), window, _ptr(prefix), _ptr(first),
+                   C.pointer(rope) if rope is not None else None)
 
 
 class SicuError(RuntimeError):
@@ -348,6 +397,42 @@ class SiphonCuda:
     def row_to_f32(self, wtype: int, dw, n_in: int, rows, dout, stream=None) -> None:
         arr = (C.c_int64 * len(rows))(*rows)
         self.check(self.lib.sicu_row_to_f32(wtype, _ptr(dw), n_in, arr, len(rows), _ptr(dout), _ptr(stream)))
+
+    # -- paged 8-bit KV cache ---------------------------------------------------------
+    def kv8_plan(self, past, fresh, n_seq: int, page: int, table, max_pages: int, free_pages, n_pages: int, n_free,
+                 n_free_out, n_tok: int, cu, length, slot, pos, stream=None) -> None:
+        """sicu_kv8_plan: a step's new pages, packed offsets, lengths, slots and positions."""
+        self.check(self.lib.sicu_kv8_plan(_ptr(past), _ptr(fresh), n_seq, page, _ptr(table), max_pages,
+                                          _ptr(free_pages), n_pages, _ptr(n_free), _ptr(n_free_out), n_tok, _ptr(cu),
+                                          _ptr(length), _ptr(slot), _ptr(pos), _ptr(stream)))
+
+    def kv8_release(self, drop, length, n_seq: int, page: int, table, max_pages: int, free_pages, n_pages: int, n_free,
+                    stream=None) -> None:
+        """sicu_kv8_release: the pages of the requests with drop != 0 become free."""
+        self.check(self.lib.sicu_kv8_release(_ptr(drop), _ptr(length), n_seq, page, _ptr(table), max_pages,
+                                             _ptr(free_pages), n_pages, _ptr(n_free), _ptr(stream)))
+
+    def kv8_store(self, cache: Kv8, type: int, dk, dv, slot, n_tok: int, pos=None, rope: RopeTables | None = None,
+                  k_stride: int = 0, v_stride: int = 0, stream=None) -> None:
+        """sicu_kv8_store: n_tok rows of K (rotated when rope is given) and V into the cache."""
+        self.check(self.lib.sicu_kv8_store(C.byref(cache), type, _ptr(dk), _ptr(dv), k_stride, v_stride, _ptr(slot),
+                                           _ptr(pos), C.byref(rope) if rope is not None else None, n_tok,
+                                           _ptr(stream)))
+
+    def kv8_load(self, cache: Kv8, type: int, slot, n_tok: int, dk, dv, stream=None) -> None:
+        """sicu_kv8_load: the stored rows of n_tok slots as values."""
+        self.check(self.lib.sicu_kv8_load(C.byref(cache), type, _ptr(slot), n_tok, _ptr(dk), _ptr(dv), _ptr(stream)))
+
+    def kv8_attention_ws(self, cache: Kv8, attn: Kv8Attn) -> int:
+        n = C.c_size_t(0)
+        self.check(self.lib.sicu_kv8_attention_ws(C.byref(cache), C.byref(attn), C.byref(n)))
+        return n.value
+
+    def kv8_attention(self, cache: Kv8, attn: Kv8Attn, dq, dout, ws=None, stream=None) -> None:
+        """sicu_kv8_attention: a step's new tokens over the cache (ws: a buffer with
+        nbytes, kv8_attention_ws bytes at least)."""
+        self.check(self.lib.sicu_kv8_attention(C.byref(cache), C.byref(attn), _ptr(dq), _ptr(dout), _ptr(ws),
+                                               ws.nbytes if ws is not None else 0, _ptr(stream)))
 
     # -- memory ---------------------------------------------------------------------
     def upload(self, host) -> int:
