@@ -7,8 +7,8 @@
 // The rows of one KV head (its n_head / n_head_kv query heads times a
 // request's new tokens) are the N side of m16n8k16 products, the cache the M
 // side: a warp takes 16 keys (one quantization block: one scale each for K
-// and V), loads their K and V codes straight into registers in an order of
-// channels and keys that makes every register an operand fragment after
+// and V) at a time from its own ring of bulk copies, loads the codes in an order
+// of channels and keys that makes every register an operand fragment after
 // byte -> f16 expansion (|code| <= 127 is exact in f16), forms S^T = K Q^T,
 // the weights in f32, and accumulates O^T += V^T P^T. Sums, maxima and the
 // output stay in f32.
@@ -27,6 +27,7 @@ constexpr int AT_WARPS = 4;
 // A new maximum rescales the accumulator only when it passes the running one
 // by 2^8: weights stay below 2^8 and f16 carries them as precisely.
 constexpr float AT_LAZY = 8.0f;
+constexpr float LOWEST = -3.402823466e38f;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -64,24 +65,25 @@ __device__ __forceinline__ float join(float mp, float m) { return mp == m ? 1.0f
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l); }
 
 template <int W>
-__device__ __forceinline__ void ldg_words(const int8_t *p, uint32_t *w) {
+__device__ __forceinline__ void lds_words(uint32_t p, uint32_t (&w)[W]) {
     if constexpr (W == 4) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint4 x = lds128(p);
         w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
     } else if constexpr (W == 2) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = x.x; w[1] = x.y;
+        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(p));
     } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        w[0] = lds32(p);
     }
 }
 
 struct AttnGeom {
     int splits;        // CTAs a request's keys may be dealt to
-    int chunk;         // keys per CTA (a multiple of 16)
+    int chunk;         // keys per CTA (a multiple of 64, at most AT_CHUNK)
     int row_tiles;     // row tiles per KV head
     int rows;          // rows kept per tile in the workspace
 };
+// A warp's keys: at most 32 blocks, one per lane's page entry and scales.
+constexpr int AT_CHUNK = AT_WARPS * 32 * KV8_BLOCK;
 
 // Partial results of one (request, KV head, row tile, split): rows x hd f32,
 // then (m, l) per row, padded to 16 bytes (the next part is written in float4s).
@@ -103,19 +105,40 @@ __device__ __forceinline__ Span tile_span(const Kv8AttnDev &a, const Kv8Seq &s, 
     return r;
 }
 
+// Blocks of a warp in flight at once: enough bytes per SM for DRAM's latency
+// (three stages of 4 KB, 16 warps) with four CTAs' rings in its shared memory.
+constexpr int AT_STAGES = 3;
+
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
+struct AttnCfg {
+    static constexpr int R = 8 * NT, KW = HD / 16, VW = HD / 32;
+    static constexpr int STAGE = 2 * KV8_BLOCK * HD;                     // K and V codes of one block
+    static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
+    static constexpr int OUT = AT_WARPS * R * HD * 4;                    // the warps' accumulators, after the ring's last use
+    static constexpr int MAIN = RING > OUT ? RING : OUT;
+    static constexpr int QROW = R * HD * 4;                              // rotated q
+    static constexpr bool Q_REGS = NT == 1 && HD <= 128;                 // q's fragments in registers, or here:
+    static constexpr int QF = Q_REGS ? 0 : KW * NT * 2 * 32 * 8;         // [word][n tile][hi, lo][lane]
+    static constexpr int SMEM = MAIN + QROW + QF;
+};
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(AT_WARPS * 32, HD * NT <= 128 ? 4 : HD * NT <= 256 ? 2 : 1)
+kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
+    using Cfg = AttnCfg<T, HD, NT>;
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int R = 8 * NT, KW = HD / 16, VW = HD / 32, WPC = HD % 64 == 0 ? 4 : 2;
+    constexpr int R = Cfg::R, KW = Cfg::KW, VW = Cfg::VW, WPC = HD % 64 == 0 ? 4 : 2;
     constexpr int VL = HD % 128 == 0 ? 4 : HD % 64 == 0 ? 2 : 1;
     constexpr int PARTS = SPLIT ? 2 : 1;        // of the weights
-    // q fragments: [word][n tile][hi, lo][lane] pairs of f16x2
-    __shared__ __align__(16) uint2 qf[KW * NT * 2 * 32];
-    __shared__ __align__(16) float qrow[R * HD];       // rotated q; the merged output later
+    extern __shared__ __align__(128) uint8_t at_sm[];
+    float *qrow = reinterpret_cast<float *>(at_sm + Cfg::MAIN);
+    uint2 *qf = reinterpret_cast<uint2 *>(at_sm + Cfg::MAIN + Cfg::QROW);
     __shared__ float rscale[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
     __shared__ int row_lo[R], row_hi[R], row_pos[R];
     __shared__ float row_slope[R];
+    __shared__ __align__(8) uint64_t bars[AT_WARPS * AT_STAGES];
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the combine, which waits for this grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
     const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, split = blockIdx.y, seq = blockIdx.z;
     const Kv8Seq s = kv8_seq(a, seq);
@@ -126,6 +149,33 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
     const int cb = g.chunk >> 4;
     const int parts = (sp.b1 - sp.b0 + cb - 1) / cb;
     if (split >= max(parts, 1)) return;
+
+    // this warp's blocks [b0, b0 + nb), nb <= 32: lane i knows block i
+    const int c0 = sp.b0 + split * cb, cn = min(cb, sp.b1 - c0), per = (cn + AT_WARPS - 1) / AT_WARPS;
+    const int b0 = c0 + warp * per, nb = max(0, min(per, c0 + cn - b0));
+    int64_t blk = 0;
+    float ks = 0.0f, vs = 0.0f;
+    if (lane < nb) {
+        blk = kv8_block(c, kv8_page(c, a, seq, b0 + lane), head, (b0 + lane) & (c.page / KV8_BLOCK - 1));
+        ks = __ldg(c.ks + blk);
+        vs = __ldg(c.vs + blk);
+    }
+    const uint32_t bar0 = smem_addr(bars + warp * AT_STAGES);
+    if (lane < AT_STAGES) mbar_init(bar0 + 8 * lane, 1);
+    fence_mbar_init();
+    __syncwarp();
+    // a ring of block copies per warp; lane i issues block i's, the first of
+    // them under q's preparation
+    const uint32_t ring = smem_addr(at_sm) + warp * (AT_STAGES * Cfg::STAGE);
+    auto issue = [&](int i) {
+        if (lane == i) {
+            const uint32_t bar = bar0 + 8 * (i % AT_STAGES), dst = ring + (i % AT_STAGES) * Cfg::STAGE;
+            mbar_expect_tx_relaxed(bar, Cfg::STAGE);
+            bulk_g2s(dst, c.k + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
+            bulk_g2s(dst + KV8_BLOCK * HD, c.v + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
+        }
+    };
+    for (int i = 0; i < AT_STAGES && i < nb; ++i) issue(i);
 
     // ---- q: rows rotated at their positions, scaled by a power of two, as fragments
     const T *q = static_cast<const T *>(a.q);
@@ -175,32 +225,43 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
         }
     }
     __syncthreads();
-    for (int i = tid; i < KW * NT * 32; i += AT_WARPS * 32) {
-        const int ln = i & 31, nt = (i >> 5) % NT, w = i / (32 * NT);
+    // the fragment words of q row nt * 8 + (ln >> 2) for k-step w
+    auto q_frag = [&](int w, int nt, int ln, uint2 &hi, uint2 &lo) {
         const int r = nt * 8 + (ln >> 2), d = (w / WPC) * (16 * WPC) + (ln & 3) * (4 * WPC) + (w % WPC) * 4;
-        const float inv = __fdiv_rn(1.0f, rscale[r]);
-        float x[4];
+        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(rscale[r]));     // 1 / a power of two
+        const float4 f = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
+        const float x0 = f.x * inv, x1 = f.y * inv, x2 = f.z * inv, x3 = f.w * inv;
+        hi = make_uint2(half2_bits(x0, x1), half2_bits(x2, x3));
+        lo = make_uint2(half2_bits(x0 - h2f(hi.x & 0xffffu), x1 - h2f(hi.x >> 16)),
+                        half2_bits(x2 - h2f(hi.y & 0xffffu), x3 - h2f(hi.y >> 16)));
+    };
+    uint2 qreg[Cfg::Q_REGS ? KW : 1][2];
+    if constexpr (Cfg::Q_REGS) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = qrow[r * HD + d + e] * inv;
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = x[e] - __half2float(__float2half_rn(x[e]));
-        qf[((w * NT + nt) * 2) * 32 + ln] = make_uint2(half2_bits(x[0], x[1]), half2_bits(x[2], x[3]));
-        qf[((w * NT + nt) * 2 + 1) * 32 + ln] = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
+        for (int w = 0; w < KW; ++w) q_frag(w, 0, lane, qreg[w][0], qreg[w][1]);
+    } else {
+        for (int i = tid; i < KW * NT * 32; i += AT_WARPS * 32) {
+            const int ln = i & 31, nt = (i >> 5) % NT, w = i / (32 * NT);
+            q_frag(w, nt, ln, qf[((w * NT + nt) * 2) * 32 + ln], qf[((w * NT + nt) * 2 + 1) * 32 + ln]);
+        }
+        __syncthreads();
     }
-    __syncthreads();
 
     // ---- keys
     // per thread: two rows (columns of the C fragment) per n tile
-    float mrun[NT][2], lsum[NT][2], rs[NT][2];
+    float mrun[NT][2], thr[NT][2], lsum[NT][2], rs[NT][2];
     float o[HD / 16][NT][4];
+    const bool mods = a.cap > 0.0f || a.slopes != nullptr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            mrun[nt][e] = -INFINITY;
+            // no key seen yet: any visible score is taken as the maximum
+            mrun[nt][e] = 0.0f;
+            thr[nt][e] = LOWEST;
             lsum[nt][e] = 0.0f;
-            rs[nt][e] = rscale[nt * 8 + 2 * tq + e] * a.scale;
+            // capped or biased scores stay in natural units until then
+            rs[nt][e] = rscale[nt * 8 + 2 * tq + e] * (float)((double)a.scale * (mods ? 1.0 : 1.4426950408889634));
         }
 #pragma unroll
     for (int mt = 0; mt < HD / 16; ++mt)
@@ -216,70 +277,85 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
         all_hi = min(all_hi, row_hi[r]);
     }
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-    const int blk_end = min(sp.b1, sp.b0 + (split + 1) * cb);
-    uint32_t kw[2][KW], vw[4][VW];
-    float ks = 0.0f, vs = 0.0f;
-    auto load = [&](int b) {
-        const int pg = kv8_page(c, a, seq, b);
-        const int64_t blk = kv8_block(c, pg, head, b & (c.page / KV8_BLOCK - 1));
-        ks = __ldg(c.ks + blk);
-        vs = __ldg(c.vs + blk);
-        const int8_t *kb = c.k + blk * (KV8_BLOCK * HD), *vb = c.v + blk * (KV8_BLOCK * HD);
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int w = 0; w < KW; w += WPC)
-                ldg_words<WPC>(kb + (gq + 8 * r) * HD + (w / WPC) * (16 * WPC) + tq * (4 * WPC), &kw[r][w]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int w = 0; w < VW; w += VL)
-                ldg_words<VL>(vb + (2 * tq + (r & 1) + 8 * (r >> 1)) * HD + gq * (HD / 8) + w * 4, &vw[r][w]);
-    };
-    int b = sp.b0 + split * cb + warp;
-    if (b < blk_end) load(b);
-    for (; b < blk_end; b += AT_WARPS) {
-        // S^T: 16 keys x R rows
-        float z[NT][4];
+    bool ok = true;
+    int i = 0, st = 0;
+    uint32_t phase = 0;
+    for (; i < nb; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * st, phase))) {
+            ok = false;
+            break;
+        }
+        const uint32_t kbuf = ring + st * Cfg::STAGE, vbuf = kbuf + KV8_BLOCK * HD;
+        const int b = b0 + i;
+        const float kscale = __shfl_sync(0xffffffffu, ks, i), vscale = __shfl_sync(0xffffffffu, vs, i);
+        // S^T: 16 keys x R rows, the parts of q in accumulators of their own
+        float z[NT][4], zl[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[nt][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) z[nt][e] = zl[nt][e] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const uint32_t x = kw[0][w] ^ 0x80808080u, y = kw[1][w] ^ 0x80808080u;
-            const uint32_t af[4] = {code_pair(x, 0x4140), code_pair(y, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4342)};
+        for (int ch = 0; ch < KW / WPC; ++ch) {
+            uint32_t k0[WPC], k1[WPC];
+            lds_words<WPC>(kbuf + gq * HD + ch * (16 * WPC) + tq * (4 * WPC), k0);
+            lds_words<WPC>(kbuf + (gq + 8) * HD + ch * (16 * WPC) + tq * (4 * WPC), k1);
+#pragma unroll
+            for (int e = 0; e < WPC; ++e) {
+                const int w = ch * WPC + e;
+                const uint32_t x = k0[e] ^ 0x80808080u, y = k1[e] ^ 0x80808080u;
+                const uint32_t af[4] = {code_pair(x, 0x4140), code_pair(y, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4342)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    uint2 f, fl;
+                    if constexpr (Cfg::Q_REGS) {
+                        f = qreg[w][0];
+                        fl = qreg[w][1];
+                    } else {
+                        f = qf[((w * NT + nt) * 2) * 32 + lane];
+                        fl = qf[((w * NT + nt) * 2 + 1) * 32 + lane];
+                    }
+                    mma_f16(z[nt], af, f.x, f.y);
+                    mma_f16(zl[nt], af, fl.x, fl.y);
+                }
+            }
+        }
+        const int j0 = b * KV8_BLOCK + gq;           // this thread's keys: j0 and j0 + 8
+        const bool masked = (b << 4) < all_lo || (b << 4) + 16 > all_hi;
+        bool grow = vscale > vref;
+        // y = z - m in powers of two; hidden keys -inf
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[nt][e] += zl[nt][e];
+        if (mods) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint2 f = qf[((w * NT + nt) * 2 + p) * 32 + lane];
-                    mma_f16(z[nt], af, f.x, f.y);
+                for (int e = 0; e < 4; ++e) {
+                    const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
+                    float x = z[nt][e] * (rs[nt][e & 1] * kscale);
+                    if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
+                    z[nt][e] = fmaf(x, LOG2E, -fmaf(row_slope[r], fabsf((float)(row_pos[r] - j)), mrun[nt][e & 1]));
+                }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[nt][e] = fmaf(z[nt][e], rs[nt][e & 1] * kscale, -mrun[nt][e & 1]);
+        }
+        if (masked) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
+                    if (j < row_lo[r] || j >= row_hi[r]) z[nt][e] = -INFINITY;
                 }
         }
-        const float kscale = ks, vscale = vs;
-        uint32_t vcur[4][VW];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vcur[r][w] = vw[r][w] ^ 0x80808080u;
-        const int j0 = b * KV8_BLOCK + gq;           // this thread's keys: j0 and j0 + 8
-        if (b + AT_WARPS < blk_end) load(b + AT_WARPS);
-        const bool masked = (b << 4) < all_lo || (b << 4) + 16 > all_hi;
-        bool grow = vscale > vref;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
-                float x = z[nt][e] * (rs[nt][e & 1] * kscale);
-                if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
-                x *= LOG2E;
-                if (a.slopes) x -= row_slope[r] * fabsf((float)(row_pos[r] - j));
-                if (masked && (j < row_lo[r] || j >= row_hi[r])) x = -INFINITY;
-                z[nt][e] = x;
-                grow |= x > mrun[nt][e & 1] + AT_LAZY;
-            }
+            for (int e = 0; e < 4; ++e) grow |= z[nt][e] > thr[nt][e & 1];
         if (__any_sync(0xffffffffu, grow)) {
             // new maxima (over the 16 keys: lanes with the same tq) and V unit
             const float vnew = fmaxf(vref, vscale), vf = vnew > 0.0f ? __fdividef(vref, vnew) : 0.0f;
@@ -288,17 +364,25 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float m = fmaxf(z[nt][e], z[nt][e + 2]);
+                    float up = fmaxf(z[nt][e], z[nt][e + 2]), f = vf;
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-                    m = fmaxf(m, mrun[nt][e]);
-                    const float f = m == -INFINITY ? 1.0f : ex2(mrun[nt][e] - m);
-                    mrun[nt][e] = m;
-                    lsum[nt][e] *= f;
+                    for (int d = 4; d < 32; d <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, d));
+                    if (thr[nt][e] == LOWEST) {
+                        if (up > LOWEST) thr[nt][e] = AT_LAZY;
+                        else up = 0.0f;
+                    } else {
+                        up = fmaxf(up, 0.0f);
+                        const float g1 = ex2(-up);
+                        lsum[nt][e] *= g1;
+                        f *= g1;
+                    }
+                    mrun[nt][e] += up;
+                    z[nt][e] -= up;
+                    z[nt][e + 2] -= up;
 #pragma unroll
                     for (int mt = 0; mt < HD / 16; ++mt) {
-                        o[mt][nt][e] *= f * vf;
-                        o[mt][nt][e + 2] *= f * vf;
+                        o[mt][nt][e] *= f;
+                        o[mt][nt][e + 2] *= f;
                     }
                 }
         }
@@ -310,35 +394,57 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float m = mrun[nt][e & 1];
-                const float p = ex2(z[nt][e] - (m == -INFINITY ? 0.0f : m));
+                const float p = ex2(z[nt][e]);
                 lsum[nt][e & 1] += p;
                 w[e] = p * vr;
             }
-            pf[nt][0][0] = movm_t(half2_bits(w[0], w[1]));
-            pf[nt][0][1] = movm_t(half2_bits(w[2], w[3]));
+            const uint32_t h0 = half2_bits(w[0], w[1]), h1 = half2_bits(w[2], w[3]);
+            pf[nt][0][0] = movm_t(h0);
+            pf[nt][0][1] = movm_t(h1);
             if constexpr (SPLIT) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] -= __half2float(__float2half_rn(w[e]));
-                pf[nt][1][0] = movm_t(half2_bits(w[0], w[1]));
-                pf[nt][1][1] = movm_t(half2_bits(w[2], w[3]));
+                pf[nt][1][0] = movm_t(half2_bits(w[0] - h2f(h0 & 0xffffu), w[1] - h2f(h0 >> 16)));
+                pf[nt][1][1] = movm_t(half2_bits(w[2] - h2f(h1 & 0xffffu), w[3] - h2f(h1 >> 16)));
             }
         }
         // O^T += V^T P^T: a word holds four channels, two per m tile
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            const uint32_t x0 = prmt(vcur[0][w], vcur[1][w], 0x5140), x1 = prmt(vcur[0][w], vcur[1][w], 0x7362);
-            const uint32_t y0 = prmt(vcur[2][w], vcur[3][w], 0x5140), y1 = prmt(vcur[2][w], vcur[3][w], 0x7362);
-            const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
-            const uint32_t hi[4] = {code_pair(x1, 0x4140), code_pair(x1, 0x4342), code_pair(y1, 0x4140), code_pair(y1, 0x4342)};
+        for (int ch = 0; ch < VW / VL; ++ch) {
+            uint32_t v0[VL], v1[VL], v2[VL], v3[VL];
+            const uint32_t vp = vbuf + 2 * tq * HD + gq * (HD / 8) + ch * (4 * VL);
+            lds_words<VL>(vp, v0);
+            lds_words<VL>(vp + HD, v1);
+            lds_words<VL>(vp + 8 * HD, v2);
+            lds_words<VL>(vp + 9 * HD, v3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int e = 0; e < VL; ++e) {
+                const int w = ch * VL + e;
+                const uint32_t p0 = v0[e] ^ 0x80808080u, p1 = v1[e] ^ 0x80808080u, p2 = v2[e] ^ 0x80808080u,
+                               p3 = v3[e] ^ 0x80808080u;
+                const uint32_t x0 = prmt(p0, p1, 0x5140), x1 = prmt(p0, p1, 0x7362);
+                const uint32_t y0 = prmt(p2, p3, 0x5140), y1 = prmt(p2, p3, 0x7362);
+                const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
+                const uint32_t hi[4] = {code_pair(x1, 0x4140), code_pair(x1, 0x4342), code_pair(y1, 0x4140), code_pair(y1, 0x4342)};
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    mma_f16(o[2 * w][nt], lo, pf[nt][p][0], pf[nt][p][1]);
-                    mma_f16(o[2 * w + 1][nt], hi, pf[nt][p][0], pf[nt][p][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        mma_f16(o[2 * w][nt], lo, pf[nt][p][0], pf[nt][p][1]);
+                        mma_f16(o[2 * w + 1][nt], hi, pf[nt][p][0], pf[nt][p][1]);
+                    }
+            }
         }
+        __syncwarp();                        // every lane has read the stage
+        if (i + AT_STAGES < nb) issue(i + AT_STAGES);
+        if (++st == AT_STAGES) {
+            st = 0;
+            phase ^= 1;
+        }
+    }
+    if (!ok) {
+        // a copy did not arrive in time: report it, and leave no copy in flight
+        if (lane == 0) atomicOr(a.status, STATUS_WAIT_TIMEOUT);
+        for (int k = i; k < min(i + AT_STAGES, nb); ++k)
+            (void)mbar_wait(bar0 + 8 * (k % AT_STAGES), (k / AT_STAGES) & 1, 200000000ull);
     }
 
     // ---- the four warps' parts, then this CTA's
@@ -350,50 +456,45 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
             if (gq == 0) {
-                sm_m[warp][nt * 8 + 2 * tq + e] = mrun[nt][e];
+                sm_m[warp][nt * 8 + 2 * tq + e] = thr[nt][e] == LOWEST ? -INFINITY : mrun[nt][e];
                 sm_l[warp][nt * 8 + 2 * tq + e] = l;
             }
         }
     if (lane == 0) sm_vr[warp] = vref;
-    __syncthreads();
-    float f[NT][2];
+    __syncthreads();                         // the rings are free: accumulators go over them
+    float *oacc = reinterpret_cast<float *>(at_sm);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = nt * 8 + 2 * tq + e;
-            float m = sm_m[0][r];
-            for (int w = 1; w < AT_WARPS; ++w) m = fmaxf(m, sm_m[w][r]);
-            f[nt][e] = join(sm_m[warp][r], m) * sm_vr[warp];
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; mt += 2)
+                *reinterpret_cast<float4 *>(oacc + (warp * R + r) * HD + gq * (HD / 8) + 2 * mt) =
+                    make_float4(o[mt][nt][e], o[mt][nt][e + 2], o[mt + 1][nt][e], o[mt + 1][nt][e + 2]);
         }
-    for (int w = 0; w < AT_WARPS; ++w) {
-        if (warp == w) {
-#pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = nt * 8 + 2 * tq + (e & 1), d = gq * (HD / 8) + 2 * mt + (e >> 1);
-                        const float x = o[mt][nt][e] * f[nt][e & 1];
-                        if (w == 0) qrow[r * HD + d] = x;
-                        else qrow[r * HD + d] += x;
-                    }
-        }
-        __syncthreads();
-    }
+    __syncthreads();
     float *part_o = ws, *part_ml = nullptr;
     if (parts > 1) {
         const int64_t pi = part_index(g, c.hkv, seq, head, rt, split);
         part_o = ws + pi * part_floats(g.rows, HD);
         part_ml = part_o + (int64_t)g.rows * HD;
     }
-    for (int i = tid; i < rows * (HD / 4); i += AT_WARPS * 32) {
-        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    for (int k = tid; k < rows * (HD / 4); k += AT_WARPS * 32) {
+        const int r = k / (HD / 4), d = (k % (HD / 4)) * 4;
         float m = sm_m[0][r], l = 0.0f;
         for (int w = 1; w < AT_WARPS; ++w) m = fmaxf(m, sm_m[w][r]);
-        for (int w = 0; w < AT_WARPS; ++w) l += sm_l[w][r] * join(sm_m[w][r], m);
-        const float4 x = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) {
+            const float f = join(sm_m[w][r], m), fv = f * sm_vr[w];
+            const float4 y = *reinterpret_cast<const float4 *>(oacc + (w * R + r) * HD + d);
+            l += sm_l[w][r] * f;
+            x.x += y.x * fv;
+            x.y += y.y * fv;
+            x.z += y.z * fv;
+            x.w += y.w * fv;
+        }
         if (parts > 1) {
             *reinterpret_cast<float4 *>(part_o + r * HD + d) = x;
             if (d == 0) {
@@ -409,39 +510,48 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv8_attn_kernel(Kv8Dev c, Kv8At
     }
 }
 
-// Joins the splits of a row in split order: one warp per row.
+// Joins the splits of a row: one CTA per row, its warps take every fourth split
+// and are added in order.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, int R, const float *ws) {
+    constexpr int E = HD / 32;
+    __shared__ float acc_sm[4][HD], l_sm[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, seq = blockIdx.z;
+    const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, r = blockIdx.y, seq = blockIdx.z;
     const Kv8Seq s = kv8_seq(a, seq);
     const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
     if (rt * R >= n_rows) return;
-    const int rows = min(R, n_rows - rt * R), r = blockIdx.y * 4 + warp;
+    const int rows = min(R, n_rows - rt * R);
     const Span sp = tile_span(a, s, rt * R / group, (rt * R + rows - 1) / group);
     const int cb = g.chunk >> 4, parts = (sp.b1 - sp.b0 + cb - 1) / cb;
     if (parts <= 1 || r >= rows) return;
     const int64_t stride = part_floats(g.rows, HD);
     const float *p0 = ws + part_index(g, c.hkv, seq, head, rt, 0) * stride;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float m = -INFINITY;
     for (int i = lane; i < parts; i += 32) m = fmaxf(m, p0[i * stride + g.rows * HD + 2 * r]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float l = 0.0f, acc[HD / 32];
+    float l = 0.0f, acc[E];
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.0f;
-    for (int i = 0; i < parts; ++i) {
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 4) {
         const float *p = p0 + i * stride;
         const float f = join(p[g.rows * HD + 2 * r], m);
         l += p[g.rows * HD + 2 * r + 1] * f;
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) acc[e] += p[r * HD + e * 32 + lane] * f;
+        for (int e = 0; e < E; ++e) acc[e] += p[r * HD + e * 32 + lane] * f;
     }
-    const float inv = inv_sum(l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc_sm[warp][e * 32 + lane] = acc[e];
+    if (lane == 0) l_sm[warp] = l;
+    __syncthreads();
+    const float inv = inv_sum(l_sm[0] + l_sm[1] + l_sm[2] + l_sm[3]);
     const int rr = rt * R + r, t = rr / group, h = head * group + rr % group;
     T *out = static_cast<T *>(a.out) + (int64_t)(s.t0 + t) * a.out_stride + (int64_t)h * HD;
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) store1(out + e * 32 + lane, acc[e] * inv);
+    for (int d = threadIdx.x; d < HD; d += 128)
+        store1(out + d, (acc_sm[0][d] + acc_sm[1][d] + acc_sm[2][d] + acc_sm[3][d]) * inv);
 }
 
 // n tiles per CTA: the rows of a request's longest piece, up to 32 (16 with
@@ -457,13 +567,17 @@ AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     AttnGeom g;
     g.row_tiles = (int)((rows + R - 1) / R);
     g.rows = (int)(rows < R ? rows : R);
-    // Keys per CTA: enough CTAs for four per SM and two rounds of them, each
-    // with at least 256 keys.
-    const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, want = 8 * (int64_t)num_sms;
+    // Keys per CTA: a CTA's preparation of q and its join cost as much as some
+    // tens of blocks, so as many keys as leave three CTAs per SM, at most a
+    // warp's 32 blocks each (2048 keys against 1024 and 512, one 131K-token
+    // request at the Qwen2.5-32B shape: 81, 99 and 125 us; 64 requests of 4250
+    // tokens at the Llama-3-8B shape: 126, 128 and 150 us), at least 256.
+    const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, want = 3 * (int64_t)num_sms;
     int64_t splits = (want + units - 1) / units;
     int64_t chunk = (a.max_len + splits - 1) / splits;
     if (chunk < 256) chunk = 256;
     chunk = (chunk + 63) / 64 * 64;
+    if (chunk > AT_CHUNK) chunk = AT_CHUNK;
     g.chunk = (int)chunk;
     // a span rounded down to a block may begin 15 keys early
     g.splits = (int)((a.max_len + 15 + chunk - 1) / chunk);
@@ -473,12 +587,22 @@ AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
 template <typename T, int HD, int NT>
 int launch_typed(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
     const dim3 grid((unsigned)(g.row_tiles * c.hkv), (unsigned)g.splits, (unsigned)a.n_seq);
-    kv8_attn_kernel<T, HD, NT><<<grid, AT_WARPS * 32, 0, st>>>(c, a, g, ws);
+    constexpr int smem = AttnCfg<T, HD, NT>::SMEM;
+    if (cudaFuncSetAttribute(kv8_attn_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return -2;
+    kv8_attn_kernel<T, HD, NT><<<grid, AT_WARPS * 32, smem, st>>>(c, a, g, ws);
     if (cudaGetLastError() != cudaSuccess) return -2;
     if (g.splits > 1) {
-        const dim3 cgrid((unsigned)(g.row_tiles * c.hkv), (unsigned)((g.rows + 3) / 4), (unsigned)a.n_seq);
-        kv8_combine_kernel<T, HD><<<cgrid, 128, 0, st>>>(c, a, g, 8 * NT, ws);
-        if (cudaGetLastError() != cudaSuccess) return -2;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(g.row_tiles * c.hkv), (unsigned)g.rows, (unsigned)a.n_seq);
+        cfg.blockDim = dim3(128);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T, HD>, c, a, g, 8 * NT, (const float *)ws) != cudaSuccess) return -2;
     }
     return 0;
 }
