@@ -21,7 +21,7 @@ ROOT = PKG.parent
 LIB = PKG / "libsiphon_cuda.so"
 
 SOURCES = ["abi.cu", "gemv.cu", "gemv_batch.cu", "gemv_f16.cu", "quantize.cu", "noalloc.cu", "prefill.cu", "allreduce.cu", "prologue.cu", "softmax.cu", "tcpeak.cu",
-           "kv8.cu", "kv8_attn.cu"]
+           "kv8.cu", "kv8_attn.cu", "kv8_prompt.cu"]
 HEADERS = ["common.cuh", "gemv.cuh", "quantize.cuh", "launch.h", "tc.cuh", "allreduce.cuh", "prologue.cuh", "kv8.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -24,6 +24,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr int AT_WARPS = 4;
+constexpr int AT_MOST = 32;
 // A new maximum rescales the accumulator only when it passes the running one
 // by 2^8: weights stay below 2^8 and f16 carries them as precisely.
 constexpr float AT_LAZY = 8.0f;
@@ -81,6 +82,7 @@ struct AttnGeom {
     int chunk;         // keys per CTA (a multiple of 64, at most AT_CHUNK)
     int row_tiles;     // row tiles per KV head
     int rows;          // rows kept per tile in the workspace
+    int most;          // requests of more rows belong to the tensor-memory kernel
 };
 // A warp's keys: at most 32 blocks, one per lane's page entry and scales.
 constexpr int AT_CHUNK = AT_WARPS * 32 * KV8_BLOCK;
@@ -143,7 +145,7 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, split = blockIdx.y, seq = blockIdx.z;
     const Kv8Seq s = kv8_seq(a, seq);
     const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
-    if (rt * R >= n_rows) return;
+    if (rt * R >= n_rows || n_rows > g.most) return;
     const int rows = min(R, n_rows - rt * R);
     const Span sp = tile_span(a, s, rt * R / group, (rt * R + rows - 1) / group);
     const int cb = g.chunk >> 4;
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a
     const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, r = blockIdx.y, seq = blockIdx.z;
     const Kv8Seq s = kv8_seq(a, seq);
     const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
-    if (rt * R >= n_rows) return;
+    if (rt * R >= n_rows || n_rows > g.most) return;
     const int rows = min(R, n_rows - rt * R);
     const Span sp = tile_span(a, s, rt * R / group, (rt * R + rows - 1) / group);
     const int cb = g.chunk >> 4, parts = (sp.b1 - sp.b0 + cb - 1) / cb;
@@ -554,17 +556,32 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a
         store1(out + d, (acc_sm[0][d] + acc_sm[1][d] + acc_sm[2][d] + acc_sm[3][d]) * inv);
 }
 
-// n tiles per CTA: the rows of a request's longest piece, up to 32 (16 with
-// 256 channels, whose accumulator would not fit the registers)
-int attn_nt(const Kv8Dev &c, const Kv8AttnDev &a) {
+// The rows (query heads of one KV head x new tokens) up to which a request
+// runs here; longer ones on the tensor-memory kernel, whose 128-row tiles few
+// rows would leave empty and whose keys are not split over CTAs. A single
+// request runs on one kernel.
+int attn_most(const Kv8Dev &c, const Kv8AttnDev &a) {
     const int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
+    if (!kv8_prompt_supported(c.hd) || rows <= AT_MOST) return INT_MAX;
+    return a.n_seq == 1 ? 0 : AT_MOST;
+}
+
+// n tiles per CTA: the rows of a request's longest piece, up to 32 (16 with
+// 256 channels, whose accumulator would not fit the registers). In a step that
+// mixes prompts with single tokens, those of one token.
+int attn_nt(const Kv8Dev &c, const Kv8AttnDev &a) {
+    const int group = a.n_head / c.hkv;
+    const int64_t rows = attn_most(c, a) == AT_MOST ? group : (int64_t)a.max_new * group;
     return rows <= 8 ? 1 : rows <= 16 || c.hd == 256 ? 2 : 4;
 }
 
 AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     const int nt = attn_nt(c, a), R = 8 * nt;
-    const int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
-    AttnGeom g;
+    AttnGeom g{};
+    g.most = attn_most(c, a);
+    if (g.most == 0) return g;               // no request runs here
+    int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
+    if (rows > g.most) rows = g.most;
     g.row_tiles = (int)((rows + R - 1) / R);
     g.rows = (int)(rows < R ? rows : R);
     // Keys per CTA: a CTA's preparation of q and its join cost as much as some
@@ -634,12 +651,16 @@ int launch_t(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws,
 size_t kv8_attn_workspace(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int num_sms) {
     (void)f16;
     const AttnGeom g = attn_geom(c, a, num_sms);
-    if (g.splits <= 1) return 0;
+    if (g.splits <= 1 || g.row_tiles == 0) return 0;
     return (size_t)a.n_seq * c.hkv * g.row_tiles * g.splits * part_floats(g.rows, c.hd) * 4;
 }
 
 int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *ws, int num_sms, cudaStream_t st) {
     const AttnGeom g = attn_geom(c, a, num_sms);
+    if (g.most != INT_MAX) {
+        if (const int rc = launch_kv8_prompt(c, a, f16, g.most, st)) return rc;
+        if (g.most == 0) return 0;
+    }
     return f16 ? launch_t<__half>(c, a, g, static_cast<float *>(ws), st)
                : launch_t<float>(c, a, g, static_cast<float *>(ws), st);
 }
