@@ -33,11 +33,8 @@ __device__ __forceinline__ void rot(float &x0, float &x1, float c, float s) {
     x1 = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
     x0 = a;
 }
-__device__ __forceinline__ void rope_oct(Oct &o, const RopeDev &r, int64_t pos, int c) {
-    if (4 * c >= r.half) return;                    // channels from n_rot on stay as they are
-    const float4 cs = __ldg(reinterpret_cast<const float4 *>(r.cs + pos * r.half + 4 * c));
-    const float4 sn = __ldg(reinterpret_cast<const float4 *>(r.sn + pos * r.half + 4 * c));
-    if (r.neox) {
+__device__ __forceinline__ void rope_oct(Oct &o, const float4 &cs, const float4 &sn, int neox) {
+    if (neox) {
         rot(o.a[0], o.b[0], cs.x, sn.x);
         rot(o.a[1], o.b[1], cs.y, sn.y);
         rot(o.a[2], o.b[2], cs.z, sn.z);
@@ -49,6 +46,30 @@ __device__ __forceinline__ void rope_oct(Oct &o, const RopeDev &r, int64_t pos, 
         rot(o.b[2], o.b[3], cs.w, sn.w);
     }
 }
+
+__device__ __forceinline__ void rope_oct(Oct &o, const RopeDev &r, int64_t pos, int c) {
+    if (4 * c >= r.half) return;                    // channels from n_rot on stay as they are
+    rope_oct(o, __ldg(reinterpret_cast<const float4 *>(r.cs + pos * r.half + 4 * c)),
+             __ldg(reinterpret_cast<const float4 *>(r.sn + pos * r.half + 4 * c)), r.neox);
+}
+
+// four consecutive values, loaded first and widened later
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+    float4 x;
+    __device__ __forceinline__ void load(const float *p) { x = __ldg(reinterpret_cast<const float4 *>(p)); }
+    __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+};
+template <>
+struct Raw4<__half> {
+    uint2 x;
+    __device__ __forceinline__ void load(const __half *p) { x = __ldg(reinterpret_cast<const uint2 *>(p)); }
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+        v[0] = h2f(x.x & 0xffffu); v[1] = h2f(x.x >> 16); v[2] = h2f(x.y & 0xffffu); v[3] = h2f(x.y >> 16);
+    }
+};
 
 // four consecutive values as f32
 __device__ __forceinline__ void load4(const float *p, float (&v)[4]) {

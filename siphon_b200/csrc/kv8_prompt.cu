@@ -33,25 +33,29 @@ constexpr float VR_MIN = 9.094947017729282e-13f;      // 2^-40: smaller relative
 constexpr uint32_t ALL = 0xffffffffu;
 
 constexpr int PT_ROWS = 256, PT_M = 128, PT_KEYS = 128, PT_BLOCKS = PT_KEYS / KV8_BLOCK;
-constexpr int PT_THREADS = 512;       // softmax 2 x 4 warps, K converters 4, MMA issue 1, V converters 3
-constexpr int PT_W_K = 8, PT_W_MMA = 12, PT_W_V = 13, PT_NV = 3;
+constexpr int PT_THREADS = 512;       // softmax 2 x 4 warps, converters 7, MMA issue 1
+constexpr int PT_W_CONV = 8, PT_W_MMA = 15, PT_NCONV = 7;
+constexpr int PT_BUF = 3;             // f16 tiles: K and V of successive key tiles take turns
 constexpr int PT_RING = 4;            // tiles whose scales are kept
 
-// barriers
-enum { B_K_FULL, B_K_FREE, B_V_FULL, B_V_FREE, B_S0, B_S1, B_P0, B_P1, B_OUT, B_DRAIN, B_SC, B_COUNT = B_SC + PT_RING };
+// Barriers. The converters fill the three tile buffers in the order K0 V0 K1
+// V1 ...: V of tile j then waits only for the scores of tile j (K's release),
+// K of tile j + 2 for the outputs of tile j, while two tiles stay in use.
+enum { B_FULL, B_FREE = B_FULL + PT_BUF, B_Q = B_FREE + PT_BUF, B_S0, B_S1, B_P0, B_P1, B_OUT, B_DRAIN, B_SC,
+       B_COUNT = B_SC + PT_RING };
 
 template <int HD>
 struct PtLay {
     static constexpr int PANELS = HD / 64, PANEL = PT_M * 128;        // 128 rows x 64 halves
     static constexpr int TILE = PANELS * PANEL;
     static constexpr int OFF_Q = 0;                                   // [tile][hi, lo]
-    static constexpr int OFF_K = OFF_Q + 4 * TILE;
-    static constexpr int OFF_V = OFF_K + TILE;
-    static constexpr int OFF_SC = OFF_V + TILE;                       // [ring][8] K scale, V factor, V term
+    static constexpr int OFF_X = OFF_Q + 4 * TILE;                    // [PT_BUF] K or V
+    static constexpr int OFF_SC = OFF_X + PT_BUF * TILE;              // [ring][8] K scale, V factor, V term
     static constexpr int OFF_RS = OFF_SC + PT_RING * PT_BLOCKS * 16;  // per-row score factor
     static constexpr int OFF_BAR = OFF_RS + PT_ROWS * 4;
     static constexpr int OFF_MISC = OFF_BAR + B_COUNT * 8;
     static constexpr int SMEM = OFF_MISC + 256 + 1024;                // base rounded up to 1024
+    static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -59,9 +63,40 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
-    const float e = ex2(x * inv_cap * (2.0f * LOG2E));
-    return cap - 2.0f * cap * __fdividef(1.0f, 1.0f + fminf(e, 1e30f));
+// two f32 in one register pair
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t dup2(float a) { return pack2(a, a); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), b, c); }
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t sel) {
     const uint32_t h = prmt(x, 0x64646464u, sel);
@@ -167,7 +202,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + Lay::OFF_MISC + 4);
     int *found = reinterpret_cast<int *>(sm + Lay::OFF_MISC + 8);             // request, tile
     int *wsum = reinterpret_cast<int *>(sm + Lay::OFF_MISC + 16);             // [16]
-    float *wmax = reinterpret_cast<float *>(sm + Lay::OFF_MISC + 80);         // [16]
+    float *wmax = reinterpret_cast<float *>(sm + Lay::OFF_MISC + 80);         // [7]
+    float *vref_sm = reinterpret_cast<float *>(sm + Lay::OFF_MISC + 144);
     float *rsv = reinterpret_cast<float *>(sm + Lay::OFF_RS);
     float4 *sc = reinterpret_cast<float4 *>(sm + Lay::OFF_SC);                // (K scale, V factor, V term, -)
     auto bar = [&](int i) { return sb + Lay::OFF_BAR + 8u * (uint32_t)i; };
@@ -225,86 +261,99 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
         return;
     }
 
-    // ---- barriers, tensor memory, the span's largest V scale, q
+    // ---- barriers and tensor memory
     if (tid == 0) {
-        mbar_init(bar(B_K_FULL), 4);
-        mbar_init(bar(B_V_FULL), PT_NV);
+        for (int i = 0; i < PT_BUF; ++i) {
+            mbar_init(bar(B_FULL + i), PT_NCONV);
+            mbar_init(bar(B_FREE + i), 1);
+        }
+        mbar_init(bar(B_Q), PT_W_CONV);
         mbar_init(bar(B_P0), 4);
         mbar_init(bar(B_P1), 4);
-        for (int i : {B_K_FREE, B_V_FREE, B_S0, B_S1, B_OUT, B_DRAIN}) mbar_init(bar(i), 1);
+        for (int i : {(int)B_S0, (int)B_S1, (int)B_OUT, (int)B_DRAIN}) mbar_init(bar(i), 1);
         for (int i = 0; i < PT_RING; ++i) mbar_init(bar(B_SC + i), 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == PT_W_MMA) tmem_alloc(smem_addr(tmem_slot), 512);
-    auto block_of = [&](int b) { return kv8_block(c, kv8_page(c, a, seq, b), head, b & (c.page / KV8_BLOCK - 1)); };
-    {
-        float m = 0.0f;
-        for (int b = b0 + tid; b < b1; b += PT_THREADS) m = fmaxf(m, __ldg(c.vs + block_of(b)));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, d));
-        if (lane == 0) wmax[warp] = m;
-    }
-    const bool mods = a.cap > 0.0f || a.slopes != nullptr;
-    const bool q_lo = SPLIT || a.rope.half > 0;
-    {
-        // OL lanes per row, one eight-channel piece each
-        constexpr int OL = HD / 8, RPW = 32 / OL;
-        const T *q = static_cast<const T *>(a.q);
-        const int o = lane % OL, neox = a.rope.neox;
-        for (int r = warp * RPW + lane / OL; r < PT_ROWS; r += PT_THREADS / 32 * RPW) {
-            Oct x;
-            if (r < rows) {
-                const int t = (r0 + r) / group, h = head * group + (r0 + r) % group;
-                const T *src = q + (int64_t)(s.t0 + t) * a.q_stride + (int64_t)h * HD;
-                load4(src + oct_a(o, neox), x.a);
-                load4(src + oct_b(o, HD, neox), x.b);
-                if (a.rope.half) {
-                    if (pos0 + t < a.rope.rows) rope_oct(x, a.rope, pos0 + t, o);
-                    else if (o == 0) atomicOr(a.status, STATUS_BAD_PLAN);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x.a[e] = x.b[e] = 0.0f;
-            }
-            float m = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
-#pragma unroll
-            for (int d = 1; d < OL; d <<= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, d));
-            // the row's largest magnitude to [1, 2) by a power of two
-            const int e2 = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
-            const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-            if (o == 0)
-                rsv[r] = __uint_as_float((uint32_t)(127 + e2) << 23) *
-                         (float)((double)a.scale * (mods ? 1.0 : 1.4426950408889634));
-            auto put = [&](int d, const float (&v)[4]) {
-                const float v0 = v[0] * inv, v1 = v[1] * inv, v2 = v[2] * inv, v3 = v[3] * inv;
-                const uint32_t h0 = half2_bits(v0, v1), h1 = half2_bits(v2, v3);
-                const int rr = r & (PT_M - 1);
-                const uint32_t at = sb + Lay::OFF_Q + (r / PT_M) * 2 * Lay::TILE + (d >> 6) * Lay::PANEL + (rr >> 3) * 1024 +
-                                    (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
-                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at), "r"(h0), "r"(h1) : "memory");
-                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at + Lay::TILE),
-                             "r"(half2_bits(v0 - h2f(h0 & 0xffffu), v1 - h2f(h0 >> 16))),
-                             "r"(half2_bits(v2 - h2f(h1 & 0xffffu), v3 - h2f(h1 >> 16))) : "memory");
-            };
-            put(oct_a(o, neox), x.a);
-            put(oct_b(o, HD, neox), x.b);
-        }
-    }
-    fence_proxy_async();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    float vref = wmax[0];
-    for (int w = 1; w < PT_THREADS / 32; ++w) vref = fmaxf(vref, wmax[w]);
+    const bool mods = a.cap > 0.0f || a.slopes != nullptr;
+    const bool q_lo = SPLIT || a.rope.half > 0;
     const uint32_t TM_S[2] = {tmem, tmem + 128}, TM_O[2] = {tmem + 256, tmem + 256 + HD};
 
-    if (warp < PT_W_K) {
+    if (warp < PT_W_CONV) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        // ---- q: OL lanes per row, one eight-channel piece each, eight rows'
+        // loads in flight
+        {
+            constexpr int OL = HD / 8, RPW = 32 / OL, STEP = PT_W_CONV * RPW, U = 8;
+            const T *q = static_cast<const T *>(a.q);
+            const int o = lane % OL, neox = a.rope.neox;
+            const bool turn = 4 * o < a.rope.half;
+            for (int rb = warp * RPW + lane / OL; rb < PT_ROWS; rb += U * STEP) {
+                Raw4<T> xa[U], xb[U];
+                float4 cs[U], sn[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    // rows past the last one repeat it: they are not written
+                    const int r = r0 + min(rb + i * STEP, rows - 1), t = r / group, h = head * group + r - t * group;
+                    const T *src = q + (int64_t)(s.t0 + t) * a.q_stride + (int64_t)h * HD;
+                    xa[i].load(src + oct_a(o, neox));
+                    xb[i].load(src + oct_b(o, HD, neox));
+                    int64_t p = pos0 + t;
+                    if (p >= a.rope.rows) {
+                        if (turn) atomicOr(a.status, STATUS_BAD_PLAN);
+                        p = 0;
+                    }
+                    if (turn) {
+                        cs[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.cs + p * a.rope.half + 4 * o));
+                        sn[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.sn + p * a.rope.half + 4 * o));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int r = rb + i * STEP;
+                    Oct x;
+                    xa[i].get(x.a);
+                    xb[i].get(x.b);
+                    if (turn) rope_oct(x, cs[i], sn[i], neox);
+                    float m = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+#pragma unroll
+                    for (int d = 1; d < OL; d <<= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, d));
+                    // the row's largest magnitude to [1, 2) by a power of two
+                    const int e2 = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
+                    const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+                    if (o == 0)
+                        rsv[r] = __uint_as_float((uint32_t)(127 + e2) << 23) *
+                                 (float)((double)a.scale * (mods ? 1.0 : 1.4426950408889634));
+                    auto put = [&](int d, const float (&v)[4]) {
+                        const float v0 = v[0] * inv, v1 = v[1] * inv, v2 = v[2] * inv, v3 = v[3] * inv;
+                        const uint32_t h0 = half2_bits(v0, v1), h1 = half2_bits(v2, v3);
+                        const int rr = r & (PT_M - 1);
+                        const uint32_t at = sb + Lay::OFF_Q + (r / PT_M) * 2 * Lay::TILE + (d >> 6) * Lay::PANEL +
+                                            (rr >> 3) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
+                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at), "r"(h0), "r"(h1) : "memory");
+                        if (q_lo)
+                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at + Lay::TILE),
+                                         "r"(half2_bits(v0 - h2f(h0 & 0xffffu), v1 - h2f(h0 >> 16))),
+                                         "r"(half2_bits(v2 - h2f(h1 & 0xffffu), v3 - h2f(h1 >> 16))) : "memory");
+                    };
+                    put(oct_a(o, neox), x.a);
+                    put(oct_b(o, HD, neox), x.b);
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_Q));
+            // the score factors are read by other warps
+            asm volatile("bar.sync 1, %0;" :: "n"(PT_W_CONV * 32) : "memory");
+        }
         // ---- weights: thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int t = warp >> 2, wq = warp & 3, r = t * PT_M + wq * 32 + lane;
         const uint32_t lanes = (uint32_t)(32 * wq) << 16;
         if (t < n_mt) {
@@ -319,7 +368,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                 wlo = max(wlo, __shfl_xor_sync(ALL, wlo, d));
                 whi = min(whi, __shfl_xor_sync(ALL, whi, d));
             }
-            const float rs = rsv[r], inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+            const float rs = rsv[r], cap_in = a.cap > 0.0f ? 1.0f / a.cap : 0.0f, cap2 = a.cap * LOG2E;
             const float slope = a.slopes ? __ldg(a.slopes + h) * LOG2E : 0.0f;
             float m = 0.0f, thr = LOWEST, l = 0.0f;
             bool ok = true;
@@ -342,20 +391,81 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                 float cb[PT_BLOCKS];
 #pragma unroll
                 for (int b = 0; b < PT_BLOCKS; ++b) cb[b] = sj[b].x * rs;
-                if (masked || mods) {
-                    // scores in place, in powers of two
+                if (mods) {
+                    // capped and biased scores in place, in powers of two
+                    if (a.cap > 0.0f) {
+                        float top = 0.0f;
+#pragma unroll
+                        for (int b = 0; b < PT_BLOCKS; ++b) {
+                            float bm = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < KV8_BLOCK; e += 2)
+                                bm = fmaxf(bm, fmaxf(fabsf(__uint_as_float(v[b >> 1][(b & 1) * 16 + e])),
+                                                     fabsf(__uint_as_float(v[b >> 1][(b & 1) * 16 + e + 1]))));
+                            top = fmaxf(top, bm * cb[b]);
+                        }
+                        if (__any_sync(ALL, !(top * cap_in <= 0.25f))) {
+                            // cap tanh x = cap - 2 cap / (1 + e^(2 x)), x = z / cap
+#pragma unroll
+                            for (int b = 0; b < PT_BLOCKS; ++b) {
+                                const float cc = cb[b] * cap_in * (2.0f * LOG2E);
+#pragma unroll
+                                for (int e = 0; e < KV8_BLOCK; ++e) {
+                                    uint32_t &u = v[b >> 1][(b & 1) * 16 + e];
+                                    u = __float_as_uint(fmaf(-2.0f * cap2, rcp(1.0f + ex2(__uint_as_float(u) * cc)), cap2));
+                                }
+                            }
+                        } else {
+                            // Scores below a quarter of the cap, as they mostly are:
+                            // the Taylor series of tanh through x^7 (the next term
+                            // is below 2^-23), two scores at a time on the FMA
+                            // pipe. The form above takes the special-function unit
+                            // twice more per score.
+#pragma unroll
+                            for (int b = 0; b < PT_BLOCKS; ++b) {
+                                const uint64_t cx = dup2(cb[b] * cap_in), cw = dup2(cb[b] * LOG2E);
+#pragma unroll
+                                for (int e = 0; e < KV8_BLOCK; e += 2) {
+                                    uint32_t &u0 = v[b >> 1][(b & 1) * 16 + e], &u1 = v[b >> 1][(b & 1) * 16 + e + 1];
+                                    const uint64_t u = pack2(__uint_as_float(u0), __uint_as_float(u1));
+                                    const uint64_t x = mul2(u, cx), y = mul2(x, x), wz = mul2(u, cw);
+                                    uint64_t g = fma2(y, dup2(-17.0f / 315.0f), dup2(2.0f / 15.0f));
+                                    g = mul2(fma2(g, y, dup2(-1.0f / 3.0f)), y);
+                                    float x0, x1;
+                                    unpack2(fma2(g, wz, wz), x0, x1);
+                                    u0 = __float_as_uint(x0);
+                                    u1 = __float_as_uint(x1);
+                                }
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < PT_BLOCKS; ++b)
+#pragma unroll
+                            for (int e = 0; e < KV8_BLOCK; ++e) {
+                                uint32_t &u = v[b >> 1][(b & 1) * 16 + e];
+                                u = __float_as_uint(__uint_as_float(u) * (cb[b] * LOG2E));
+                            }
+                    }
+#pragma unroll
+                    for (int b = 0; b < PT_BLOCKS; ++b) cb[b] = 1.0f;
+                    if (a.slopes) {
+                        const float dist = (float)(p - k0);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[q][e] = __float_as_uint(fmaf(-slope, fabsf(dist - (float)(q * 32 + e)), __uint_as_float(v[q][e])));
+                    }
+                }
+                if (masked) {
 #pragma unroll
                     for (int b = 0; b < PT_BLOCKS; ++b) {
 #pragma unroll
                         for (int e = 0; e < KV8_BLOCK; ++e) {
                             uint32_t &u = v[b >> 1][(b & 1) * 16 + e];
                             const int key = k0 + b * KV8_BLOCK + e;
-                            float x = __uint_as_float(u) * cb[b];
-                            if (mods) {
-                                if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
-                                x = fmaf(x, LOG2E, -slope * fabsf((float)(p - key)));
-                            }
-                            u = __float_as_uint(key < rlo || key >= rhi ? -INFINITY : x);
+                            u = __float_as_uint(key < rlo || key >= rhi ? -INFINITY : __uint_as_float(u) * cb[b]);
                         }
                         cb[b] = 1.0f;
                     }
@@ -363,10 +473,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                 float mx = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < PT_BLOCKS; ++b) {
-                    float bm = __uint_as_float(v[b >> 1][(b & 1) * 16]);
-#pragma unroll
-                    for (int e = 1; e < KV8_BLOCK; ++e) bm = fmaxf(bm, __uint_as_float(v[b >> 1][(b & 1) * 16 + e]));
-                    mx = fmaxf(mx, bm * cb[b]);
+                    const uint32_t *u = &v[b >> 1][(b & 1) * 16];
+                    float bm = max3(u[0], u[1], u[2]), bn = max3(u[3], u[4], u[5]);
+                    bm = max3(bm, u[6], u[7]);
+                    bn = max3(bn, u[8], u[9]);
+                    bm = max3(bm, u[10], u[11]);
+                    bn = max3(bn, u[12], u[13]);
+                    bm = max3(bm, u[14], u[15]);
+                    mx = fmaxf(mx, fmaxf(bm, bn) * cb[b]);
                 }
                 const bool grow = mx > thr;
                 if (__any_sync(ALL, grow)) {
@@ -400,14 +514,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                         // the relative scale) and leaves the sum by its inverse;
                         // f32: a product of its own, exact to 2^-24
                         const float2 fb = make_float2(sj[b].y, sj[b].z);
-                        const float sub = SPLIT ? m : m - fb.y;
-                        float sum = 0.0f;
+                        const float sub = SPLIT ? -m : fb.y - m;
+                        const uint64_t c2 = pack2(cb[b], cb[b]), s2 = pack2(sub, sub);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int e = 0; e < KV8_BLOCK; e += 2) {
-                            const float x0 = ex2(fmaf(__uint_as_float(v[q][hb * 16 + e]), cb[b], -sub));
-                            const float x1 = ex2(fmaf(__uint_as_float(v[q][hb * 16 + e + 1]), cb[b], -sub));
-                            sum += x0;
-                            sum += x1;
+                            float x0, x1;
+                            unpack2(fma2(pack2(__uint_as_float(v[q][hb * 16 + e]), __uint_as_float(v[q][hb * 16 + e + 1])), c2, s2), x0, x1);
+                            x0 = ex2(x0);
+                            x1 = ex2(x1);
+                            sum = add2(sum, pack2(x0, x1));
                             if constexpr (SPLIT) {
                                 const float w0 = x0 * fb.x, w1 = x1 * fb.x;
                                 const uint32_t hw = half2_bits(w0, w1);
@@ -417,7 +533,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                                 ph[hb * 8 + e / 2] = half2_bits(x0, x1);
                             }
                         }
-                        l += SPLIT ? sum : sum * fb.x;
+                        float l0, l1;
+                        unpack2(sum, l0, l1);
+                        l += SPLIT ? l0 + l1 : (l0 + l1) * fb.x;
                     }
                     tmem_st16(ts + 16 * q, ph);
                     if constexpr (SPLIT) tmem_st16(ts + 64 + 16 * q, pl);
@@ -429,76 +547,149 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             }
             if (ok && __all_sync(ALL, pt_wait<true>(bar(B_OUT), 0, abort_flag, a.status))) {
                 tc_fence_after();
-                const float f = l == 0.0f ? 0.0f : __fdiv_rn(vref, l);
-                const int rr = r0 + r;
-                T *dst = out + (int64_t)(s.t0 + rr / group) * a.out_stride + (int64_t)(head * group + rr % group) * HD;
+                const float f = l == 0.0f ? 0.0f : __fdiv_rn(*vref_sm, l);
+                // through this warp's part of q's shared memory (every product
+                // has ended), so that rows are written whole: 16-byte units,
+                // turned by the row against bank conflicts
+                constexpr int UNITS = HD * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
+                const uint32_t mine = sb + Lay::OFF_Q + warp * (32 * HD * 4);
 #pragma unroll
                 for (int q = 0; q < HD; q += 32) {
                     uint32_t w[32];
                     tmem_ld32(to + q, w);
                     tmem_wait_all();
                     tie32(w);
-                    if (live) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            store4(dst + q + e, __uint_as_float(w[e]) * f, __uint_as_float(w[e + 1]) * f,
-                                   __uint_as_float(w[e + 2]) * f, __uint_as_float(w[e + 3]) * f);
+                    for (int e = 0; e < 32; e += PER) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (SPLIT) x[i] = __float_as_uint(__uint_as_float(w[e + i]) * f);
+                            else x[i] = half2_bits(__uint_as_float(w[e + 2 * i]) * f, __uint_as_float(w[e + 2 * i + 1]) * f);
+                        }
+                        sts128(mine + (lane * UNITS + (((q + e) / PER) ^ (lane & 7))) * 16, x[0], x[1], x[2], x[3]);
                     }
+                }
+                __syncwarp();
+                const int tok = (r0 + r) / group;
+                const int64_t row_at = (int64_t)(s.t0 + tok) * a.out_stride + (int64_t)(head * group + r0 + r - tok * group) * HD;
+#pragma unroll 4
+                for (int i = lane; i < 32 * UNITS; i += 32) {
+                    const int rw = i / UNITS, u = i % UNITS;
+                    const int64_t at = __shfl_sync(ALL, row_at, rw);
+                    const uint4 x = lds128(mine + (rw * UNITS + (u ^ (rw & 7))) * 16);
+                    if (t * PT_M + wq * 32 + rw < rows) *reinterpret_cast<uint4 *>(out + at + u * PER) = x;
                 }
             }
         }
     } else {
-      // one instruction for each whole warpgroup: 256 x 176 + 256 x 80
+      // one instruction for each whole warpgroup: 256 x 184 + 256 x 72
       // registers are the launch's 512 x 128
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp < PT_W_MMA) {
-        // ---- K: codes to f16, and the tile's scales
-        constexpr int N = Piece<HD>::COUNT / 4;
-        const int w = warp - PT_W_K;
+        // ---- codes to f16, and the tiles' scales
+        constexpr int N = (Piece<HD>::COUNT + PT_NCONV - 1) / PT_NCONV;
+        const int w = warp - PT_W_CONV;
+        auto block_of = [&](int b) { return kv8_block(c, kv8_page(c, a, seq, b), head, b & (c.page / KV8_BLOCK - 1)); };
         uint4 piece[N];
+        // of the tile being fetched: lane i < 8 its block i (-1 past the span);
+        // of the one after it: the page id, read a tile ahead so that no fetch
+        // waits for the table
         int64_t blk = -1;
+        int page = -1;
         float ksc = 0.0f, vsc = 0.0f;
-        auto fetch = [&](int j) {
+        auto find_page = [&](int j) {
+            const int b = b0 + j * PT_BLOCKS + lane;
+            page = lane < PT_BLOCKS && b < b1 ? __ldg(a.table + (int64_t)seq * a.max_pages + (b >> (c.page_shift - 4))) : -1;
+        };
+        auto find_blocks = [&](int j) {
             const int b = b0 + j * PT_BLOCKS + lane;
             blk = -1;
-            ksc = vsc = 0.0f;
             if (lane < PT_BLOCKS && b < b1) {
-                blk = block_of(b);
-                if (w == 0) {
-                    ksc = __ldg(c.ks + blk);
-                    vsc = __ldg(c.vs + blk);
+                if ((unsigned)page >= (unsigned)c.n_pages) {
+                    atomicOr(a.status, STATUS_BAD_PLAN);
+                    page = 0;
                 }
+                blk = kv8_block(c, page, head, b & (c.page / KV8_BLOCK - 1));
             }
+            find_page(j + 1);
+        };
+        auto fetch = [&](const int8_t *codes) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int u = w + 4 * i;
-                piece[i] = piece_load<HD>(c.k, __shfl_sync(ALL, blk, u * Piece<HD>::ROWS / KV8_BLOCK), u, lane);
+                const int u = w + PT_NCONV * i;
+                const int64_t mine = __shfl_sync(ALL, blk, min(u, Piece<HD>::COUNT - 1) * Piece<HD>::ROWS / KV8_BLOCK);
+                if (u < Piece<HD>::COUNT) piece[i] = piece_load<HD>(codes, mine, u, lane);
             }
         };
-        fetch(0);
-        for (int j = 0; j < nj; ++j) {
-            if (!__all_sync(ALL, pt_wait(bar(B_K_FREE), (uint32_t)(j & 1) ^ 1u, abort_flag, a.status))) break;
+        auto fetch_scales = [&]() {
+            ksc = w == 0 && blk >= 0 ? __ldg(c.ks + blk) : 0.0f;
+            vsc = w == 0 && blk >= 0 ? __ldg(c.vs + blk) : 0.0f;
+        };
+        find_page(0);
+        find_blocks(0);
+        fetch(c.k);
+        fetch_scales();
+        // the span's largest V scale: the unit of the accumulator
+        float vref = 0.0f;
+        for (int b = b0 + w * 32 + lane; b < b1; b += PT_NCONV * 32) vref = fmaxf(vref, __ldg(c.vs + block_of(b)));
 #pragma unroll
-            for (int i = 0; i < N; ++i) piece_store<HD>(sb + Lay::OFF_K, piece[i], w + 4 * i, lane);
-            if (w == 0 && lane < PT_BLOCKS) {
+        for (int d = 16; d; d >>= 1) vref = fmaxf(vref, __shfl_xor_sync(ALL, vref, d));
+        if (lane == 0) wmax[w] = vref;
+        asm volatile("bar.sync 2, %0;" :: "n"(PT_NCONV * 32) : "memory");
+        for (int i = 0; i < PT_NCONV; ++i) vref = fmaxf(vref, wmax[i]);
+        if (w == 0 && lane == 0) *vref_sm = vref;
+        int buf = 0;
+        uint32_t phase = 1;
+        bool ok = true;
+        // the fetched tile into the next buffer
+        auto put = [&](int sc_entry) {
+            ok = __all_sync(ALL, pt_wait(bar(B_FREE + buf), phase, abort_flag, a.status));
+            if (!ok) return;
+            const uint32_t tile = sb + Lay::OFF_X + buf * Lay::TILE;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (w + PT_NCONV * i < Piece<HD>::COUNT) piece_store<HD>(tile, piece[i], w + PT_NCONV * i, lane);
+            if (sc_entry >= 0 && w == 0 && lane < PT_BLOCKS) {
                 const float vr = vref > 0.0f ? fmaxf(__fdiv_rn(vsc, vref), VR_MIN) : 1.0f;
-                sc[(j % PT_RING) * PT_BLOCKS + lane] =
+                sc[sc_entry * PT_BLOCKS + lane] =
                     SPLIT ? make_float4(ksc, vr, 0.0f, 0.0f) : make_float4(ksc, __fdiv_rn(1.0f, vr), __log2f(vr), 0.0f);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(bar(B_K_FULL));
-                if (w == 0) mbar_arrive(bar(B_SC + j % PT_RING));
+                mbar_arrive(bar(B_FULL + buf));
+                if (sc_entry >= 0 && w == 0) mbar_arrive(bar(B_SC + sc_entry));
             }
-            if (j + 1 < nj) fetch(j + 1);
+            if (++buf == PT_BUF) {
+                buf = 0;
+                phase ^= 1;
+            }
+        };
+        for (int j = 0; j < nj; ++j) {
+            // a tile's codes travel while the other kind's are converted; two
+            // sets of registers would spill
+            put(j % PT_RING);
+            if (!ok) break;
+            fetch(c.v);
+            put(-1);
+            if (!ok) break;
+            if (j + 1 < nj) {
+                find_blocks(j + 1);
+                fetch(c.k);
+                fetch_scales();
+            }
         }
-      } else if (warp == PT_W_MMA) {
+      } else {
         // ---- MMA issue
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_f16_f32(PT_M, PT_KEYS), id_o = idesc_f16_f32(PT_M, HD) | (1u << 16);
-            auto scores = [&](int t) {
-                const uint32_t q = sb + Lay::OFF_Q + t * 2 * Lay::TILE, k = sb + Lay::OFF_K;
+            // tile buffers in the converters' order: K of tile j is the 2 j th, V the 2 j + 1 th
+            auto x_buf = [&](int n) { return n % PT_BUF; };
+            auto x_par = [&](int n) { return (uint32_t)(n / PT_BUF) & 1u; };
+            auto x_at = [&](int n) { return sb + Lay::OFF_X + x_buf(n) * Lay::TILE; };
+            auto scores = [&](int t, int j) {
+                const uint32_t q = sb + Lay::OFF_Q + t * 2 * Lay::TILE, k = x_at(2 * j);
                 for (int part = 0; part < (q_lo ? 2 : 1); ++part)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
@@ -507,31 +698,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                                    smem_desc(k + off, 1024, SMEM_SWZ_128B), id_s, (part | kk) != 0);
                     }
                 tc_commit(bar(B_S0 + t));
+                if (t == n_mt - 1) tc_commit(bar(B_FREE + x_buf(2 * j)));
             };
-            bool ok = pt_wait<true>(bar(B_K_FULL), 0, abort_flag, a.status);
+            auto full = [&](int n) { return pt_wait<true>(bar(B_FULL + x_buf(n)), x_par(n), abort_flag, a.status); };
+            bool ok = pt_wait<true>(bar(B_Q), 0, abort_flag, a.status) && full(0);
             if (ok) {
                 tc_fence_after();
-                for (int t = 0; t < n_mt; ++t) scores(t);
-                tc_commit(bar(B_K_FREE));
+                for (int t = 0; t < n_mt; ++t) scores(t, 0);
             }
             for (int j = 0; ok && j < nj; ++j) {
-                for (int t = 0; ok && t < n_mt; ++t) {
-                    if (t == 0) ok = pt_wait<true>(bar(B_V_FULL), (uint32_t)j & 1u, abort_flag, a.status);
+                for (int t = 0; t < n_mt; ++t) {
+                    if (t == 0) ok = full(2 * j + 1);
                     ok = ok && pt_wait<true>(bar(B_P0 + t), (uint32_t)j & 1u, abort_flag, a.status);
                     if (!ok) break;
                     tc_fence_after();
+                    const uint32_t v = x_at(2 * j + 1);
                     for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
                         for (int kk = 0; kk < PT_KEYS / 16; ++kk)
-                            tc_mma_f16_ts(TM_O[t], TM_S[t] + 64 * part + 8 * kk,
-                                          v_desc(sb + Lay::OFF_V + kk * 2048, Lay::PANEL), id_o, (j | part | kk) != 0);
-                    if (t == n_mt - 1) tc_commit(j + 1 < nj ? bar(B_V_FREE) : bar(B_OUT));
+                            tc_mma_f16_ts(TM_O[t], TM_S[t] + 64 * part + 8 * kk, v_desc(v + kk * 2048, Lay::PANEL), id_o,
+                                          (j | part | kk) != 0);
+                    if (t == n_mt - 1) tc_commit(j + 1 < nj ? bar(B_FREE + x_buf(2 * j + 1)) : bar(B_OUT));
                     if (j + 1 < nj) {
-                        if (t == 0) ok = pt_wait<true>(bar(B_K_FULL), (uint32_t)(j + 1) & 1u, abort_flag, a.status);
+                        if (t == 0) ok = full(2 * j + 2);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(t);
-                        if (t == n_mt - 1) tc_commit(bar(B_K_FREE));
+                        scores(t, j + 1);
                     }
                 }
             }
@@ -540,33 +732,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                 tc_commit(bar(B_DRAIN));
                 (void)mbar_wait(bar(B_DRAIN), 0, 200000000ull);
             }
-        }
-      } else {
-        // ---- V: codes to f16
-        constexpr int N = (Piece<HD>::COUNT + PT_NV - 1) / PT_NV;
-        const int w = warp - PT_W_V;
-        uint4 piece[N];
-        auto fetch = [&](int j) {
-            const int b = b0 + j * PT_BLOCKS + lane;
-            int64_t blk = -1;
-            if (lane < PT_BLOCKS && b < b1) blk = block_of(b);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int u = w + PT_NV * i;
-                const int64_t mine = __shfl_sync(ALL, blk, min(u, Piece<HD>::COUNT - 1) * Piece<HD>::ROWS / KV8_BLOCK);
-                if (u < Piece<HD>::COUNT) piece[i] = piece_load<HD>(c.v, mine, u, lane);
-            }
-        };
-        fetch(0);
-        for (int j = 0; j < nj; ++j) {
-            if (!__all_sync(ALL, pt_wait(bar(B_V_FREE), (uint32_t)(j & 1) ^ 1u, abort_flag, a.status))) break;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (w + PT_NV * i < Piece<HD>::COUNT) piece_store<HD>(sb + Lay::OFF_V, piece[i], w + PT_NV * i, lane);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_V_FULL));
-            if (j + 1 < nj) fetch(j + 1);
         }
       }
     }
