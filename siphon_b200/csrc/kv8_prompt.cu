@@ -143,6 +143,28 @@ __device__ __forceinline__ void tie32(uint32_t (&v)[32]) {
                  :: "memory");
 }
 
+// the MMAs and commits of a warp: lanes with one != 0 issue
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 :: "r"(bar), "r"(one) : "memory");
+}
+
 // Shared-memory descriptor of V as the N side of O += P V: the keys are the
 // K dimension, so N (channels) is the contiguous one. 64 channels of 8 keys
 // make one 1024-byte swizzle atom; the next 8 keys follow it (stride offset),
@@ -681,58 +703,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             }
         }
       } else {
-        // ---- MMA issue
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_f16_f32(PT_M, PT_KEYS), id_o = idesc_f16_f32(PT_M, HD) | (1u << 16);
-            // tile buffers in the converters' order: K of tile j is the 2 j th, V the 2 j + 1 th
-            auto x_buf = [&](int n) { return n % PT_BUF; };
-            auto x_par = [&](int n) { return (uint32_t)(n / PT_BUF) & 1u; };
-            auto x_at = [&](int n) { return sb + Lay::OFF_X + x_buf(n) * Lay::TILE; };
-            auto scores = [&](int t, int j) {
-                const uint32_t q = sb + Lay::OFF_Q + t * 2 * Lay::TILE, k = x_at(2 * j);
-                for (int part = 0; part < (q_lo ? 2 : 1); ++part)
+        // ---- MMA issue: the whole warp walks the loop, so that descriptors
+        // stay in uniform registers (formed by one lane they cost more than
+        // the 64 cycles of an MMA), and one elected lane issues
+        constexpr uint32_t id_s = idesc_f16_f32(PT_M, PT_KEYS), id_o = idesc_f16_f32(PT_M, HD) | (1u << 16);
+        const uint32_t one = elect_one();
+        // tile buffers in the converters' order: K of tile j is the 2 j th, V the 2 j + 1 th
+        auto x_buf = [&](int n) { return n % PT_BUF; };
+        auto x_par = [&](int n) { return (uint32_t)(n / PT_BUF) & 1u; };
+        auto x_at = [&](int n) { return sb + Lay::OFF_X + x_buf(n) * Lay::TILE; };
+        auto wait = [&](int b, uint32_t parity) { return __all_sync(ALL, pt_wait<true>(bar(b), parity, abort_flag, a.status)); };
+        auto full = [&](int n) { return wait(B_FULL + x_buf(n), x_par(n)); };
+        auto scores = [&](int t, int j) {
+            const uint64_t q = smem_desc(sb + Lay::OFF_Q + t * 2 * Lay::TILE, 1024, SMEM_SWZ_128B);
+            const uint64_t k = smem_desc(x_at(2 * j), 1024, SMEM_SWZ_128B);
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint32_t off = (kk / 4) * Lay::PANEL + (kk % 4) * 32;
-                        tc_mma_f16(TM_S[t], smem_desc(q + part * Lay::TILE + off, 1024, SMEM_SWZ_128B),
-                                   smem_desc(k + off, 1024, SMEM_SWZ_128B), id_s, (part | kk) != 0);
-                    }
-                tc_commit(bar(B_S0 + t));
-                if (t == n_mt - 1) tc_commit(bar(B_FREE + x_buf(2 * j)));
-            };
-            auto full = [&](int n) { return pt_wait<true>(bar(B_FULL + x_buf(n)), x_par(n), abort_flag, a.status); };
-            bool ok = pt_wait<true>(bar(B_Q), 0, abort_flag, a.status) && full(0);
-            if (ok) {
-                tc_fence_after();
-                for (int t = 0; t < n_mt; ++t) scores(t, 0);
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t off = ((kk / 4) * Lay::PANEL + (kk % 4) * 32) >> 4;
+                mma_ss(one, TM_S[t], q + off, k + off, id_s, kk != 0);
             }
-            for (int j = 0; ok && j < nj; ++j) {
-                for (int t = 0; t < n_mt; ++t) {
-                    if (t == 0) ok = full(2 * j + 1);
-                    ok = ok && pt_wait<true>(bar(B_P0 + t), (uint32_t)j & 1u, abort_flag, a.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v = x_at(2 * j + 1);
-                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+            if (q_lo) {
 #pragma unroll
-                        for (int kk = 0; kk < PT_KEYS / 16; ++kk)
-                            tc_mma_f16_ts(TM_O[t], TM_S[t] + 64 * part + 8 * kk, v_desc(v + kk * 2048, Lay::PANEL), id_o,
-                                          (j | part | kk) != 0);
-                    if (t == n_mt - 1) tc_commit(j + 1 < nj ? bar(B_FREE + x_buf(2 * j + 1)) : bar(B_OUT));
-                    if (j + 1 < nj) {
-                        if (t == 0) ok = full(2 * j + 2);
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(t, j + 1);
-                    }
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t off = ((kk / 4) * Lay::PANEL + (kk % 4) * 32) >> 4;
+                    mma_ss(one, TM_S[t], q + (Lay::TILE >> 4) + off, k + off, id_s, 1);
                 }
             }
-            if (*abort_flag) {
-                // every product issued must end before shared and tensor memory go
-                tc_commit(bar(B_DRAIN));
-                (void)mbar_wait(bar(B_DRAIN), 0, 200000000ull);
+            commit(one, bar(B_S0 + t));
+            if (t == n_mt - 1) commit(one, bar(B_FREE + x_buf(2 * j)));
+        };
+        bool ok = wait(B_Q, 0) && full(0);
+        if (ok) {
+            tc_fence_after();
+            for (int t = 0; t < n_mt; ++t) scores(t, 0);
+        }
+        for (int j = 0; ok && j < nj; ++j) {
+            const uint64_t v = v_desc(x_at(2 * j + 1), Lay::PANEL);
+            for (int t = 0; t < n_mt; ++t) {
+                if (t == 0) ok = full(2 * j + 1);
+                ok = ok && wait(B_P0 + t, (uint32_t)j & 1u);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                    for (int kk = 0; kk < PT_KEYS / 16; ++kk)
+                        mma_ts(one, TM_O[t], TM_S[t] + 64 * part + 8 * kk, v + (uint32_t)(kk * 2048 >> 4), id_o,
+                               part | kk ? 1u : (uint32_t)(j != 0));
+                if (t == n_mt - 1) commit(one, j + 1 < nj ? bar(B_FREE + x_buf(2 * j + 1)) : bar(B_OUT));
+                if (j + 1 < nj) {
+                    if (t == 0) ok = full(2 * j + 2);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(t, j + 1);
+                }
             }
         }
+        if (*abort_flag) {
+            // every product issued must end before shared and tensor memory go
+            commit(one, bar(B_DRAIN));
+            (void)mbar_wait(bar(B_DRAIN), 0, 200000000ull);
+        }
+        __syncwarp();
       }
     }
 
