@@ -658,7 +658,7 @@ size_t kv8_attn_workspace(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int nu
 int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *ws, int num_sms, cudaStream_t st) {
     const AttnGeom g = attn_geom(c, a, num_sms);
     if (g.most != INT_MAX) {
-        if (const int rc = launch_kv8_prompt(c, a, f16, g.most, st)) return rc;
+        if (const int rc = launch_kv8_prompt(c, a, f16, g.most, num_sms, st)) return rc;
         if (g.most == 0) return 0;
     }
     return f16 ? launch_t<__half>(c, a, g, static_cast<float *>(ws), st)

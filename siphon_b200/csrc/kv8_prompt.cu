@@ -41,7 +41,7 @@ constexpr int PT_RING = 4;            // tiles whose scales are kept
 // Barriers. The converters fill the three tile buffers in the order K0 V0 K1
 // V1 ...: V of tile j then waits only for the scores of tile j (K's release),
 // K of tile j + 2 for the outputs of tile j, while two tiles stay in use.
-enum { B_FULL, B_FREE = B_FULL + PT_BUF, B_Q = B_FREE + PT_BUF, B_S0, B_S1, B_P0, B_P1, B_OUT, B_DRAIN, B_SC,
+enum { B_FULL, B_FREE = B_FULL + PT_BUF, B_S0 = B_FREE + PT_BUF, B_S1, B_P0, B_P1, B_OUT, B_DRAIN, B_SC,
        B_COUNT = B_SC + PT_RING };
 
 template <int HD>
@@ -208,6 +208,7 @@ struct PtParams {
     Kv8Dev c;
     Kv8AttnDev a;
     int skip_rows;        // requests of at most this many rows belong to the other kernel
+    int tile_rows;        // rows per CTA: 256, or 128 (one tile) when that leaves SMs idle
 };
 
 template <typename T, int HD>
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
         if (i0 + tid < a.n_seq) {
             const Kv8Seq s = kv8_seq(a, i0 + tid);
             const int rows = s.n_new * group;
-            if (rows > prm.skip_rows) n = (rows + PT_ROWS - 1) / PT_ROWS;
+            if (rows > prm.skip_rows) n = (rows + prm.tile_rows - 1) / prm.tile_rows;
         }
         int x = n;
 #pragma unroll
@@ -265,9 +266,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
     }
     __syncthreads();
     if (found[0] < 0) return;
-    const int seq = found[0], r0 = found[1] * PT_ROWS;
+    const int seq = found[0], r0 = found[1] * prm.tile_rows;
     const Kv8Seq s = kv8_seq(a, seq);
-    const int rows = min(PT_ROWS, s.n_new * group - r0), pos0 = s.len - s.n_new;
+    const int rows = min(prm.tile_rows, s.n_new * group - r0), pos0 = s.len - s.n_new;
     const int n_mt = rows > PT_M ? 2 : 1;
     const int lo = kv8_lo(a, s, pos0 + r0 / group), hi = kv8_hi(s, pos0 + (r0 + rows - 1) / group);
     const int b0 = lo >> 4, b1 = lo < hi ? (hi + 15) >> 4 : b0;
@@ -289,7 +290,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             mbar_init(bar(B_FULL + i), PT_NCONV);
             mbar_init(bar(B_FREE + i), 1);
         }
-        mbar_init(bar(B_Q), PT_W_CONV);
         mbar_init(bar(B_P0), 4);
         mbar_init(bar(B_P1), 4);
         for (int i : {(int)B_S0, (int)B_S1, (int)B_OUT, (int)B_DRAIN}) mbar_init(bar(i), 1);
@@ -298,83 +298,125 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
         fence_mbar_init();
     }
     if (warp == PT_W_MMA) tmem_alloc(smem_addr(tmem_slot), 512);
+    const bool mods = a.cap > 0.0f || a.slopes != nullptr;
+    const bool q_lo = SPLIT || a.rope.half > 0;
+
+    // ---- converters: the first tile's codes on their way
+    constexpr int NP = (Piece<HD>::COUNT + PT_NCONV - 1) / PT_NCONV;
+    const int cw = warp - PT_W_CONV;
+    uint4 piece[NP];
+    // of the tile being fetched: lane i < 8 its block i (-1 past the span); of
+    // the one after it: the page id, read a tile ahead so that no fetch waits
+    // for the table
+    int64_t blk = -1;
+    int page = -1;
+    float ksc = 0.0f, vsc = 0.0f;
+    auto find_page = [&](int j) {
+        const int b = b0 + j * PT_BLOCKS + lane;
+        page = lane < PT_BLOCKS && b < b1 ? __ldg(a.table + (int64_t)seq * a.max_pages + (b >> (c.page_shift - 4))) : -1;
+    };
+    auto find_blocks = [&](int j) {
+        const int b = b0 + j * PT_BLOCKS + lane;
+        blk = -1;
+        if (lane < PT_BLOCKS && b < b1) {
+            if ((unsigned)page >= (unsigned)c.n_pages) {
+                atomicOr(a.status, STATUS_BAD_PLAN);
+                page = 0;
+            }
+            blk = kv8_block(c, page, head, b & (c.page / KV8_BLOCK - 1));
+        }
+        find_page(j + 1);
+    };
+    auto fetch = [&](const int8_t *codes) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int u = cw + PT_NCONV * i;
+            const int64_t mine = __shfl_sync(ALL, blk, min(u, Piece<HD>::COUNT - 1) * Piece<HD>::ROWS / KV8_BLOCK);
+            if (u < Piece<HD>::COUNT) piece[i] = piece_load<HD>(codes, mine, u, lane);
+        }
+    };
+    auto fetch_scales = [&]() {
+        ksc = cw == 0 && blk >= 0 ? __ldg(c.ks + blk) : 0.0f;
+        vsc = cw == 0 && blk >= 0 ? __ldg(c.vs + blk) : 0.0f;
+    };
+    if (warp >= PT_W_CONV && warp < PT_W_MMA) {
+        find_page(0);
+        find_blocks(0);
+        fetch(c.k);
+        fetch_scales();
+    }
+
+    // ---- q: all warps, OL lanes per row, one eight-channel piece each, four
+    // rows' loads in flight
+    {
+        constexpr int OL = HD / 8, RPW = 32 / OL, STEP = PT_THREADS / 32 * RPW, U = 4;
+        const T *q = static_cast<const T *>(a.q);
+        const int o = lane % OL, neox = a.rope.neox;
+        const bool turn = 4 * o < a.rope.half;
+        const float unit = (float)((double)a.scale * (mods ? 1.0 : 1.4426950408889634));
+        for (int rb = warp * RPW + lane / OL; rb < n_mt * PT_M; rb += U * STEP) {
+            Raw4<T> xa[U], xb[U];
+            float4 cs[U], sn[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                // rows past the last one repeat it: they are not written
+                const int r = r0 + min(rb + i * STEP, rows - 1), t = r / group, h = head * group + r - t * group;
+                const T *src = q + (int64_t)(s.t0 + t) * a.q_stride + (int64_t)h * HD;
+                xa[i].load(src + oct_a(o, neox));
+                xb[i].load(src + oct_b(o, HD, neox));
+                int64_t p = pos0 + t;
+                if (p >= a.rope.rows) {
+                    if (turn) atomicOr(a.status, STATUS_BAD_PLAN);
+                    p = 0;
+                }
+                if (turn) {
+                    cs[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.cs + p * a.rope.half + 4 * o));
+                    sn[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.sn + p * a.rope.half + 4 * o));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int r = rb + i * STEP;
+                Oct x;
+                xa[i].get(x.a);
+                xb[i].get(x.b);
+                if (turn) rope_oct(x, cs[i], sn[i], neox);
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+#pragma unroll
+                for (int d = 1; d < OL; d <<= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, d));
+                // the row's largest magnitude to [1, 2) by a power of two
+                const int e2 = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
+                const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+                if (o == 0) rsv[r] = __uint_as_float((uint32_t)(127 + e2) << 23) * unit;
+                auto put = [&](int d, const float (&v)[4]) {
+                    const float v0 = v[0] * inv, v1 = v[1] * inv, v2 = v[2] * inv, v3 = v[3] * inv;
+                    const __half2 h0 = __floats2half2_rn(v0, v1), h1 = __floats2half2_rn(v2, v3);
+                    const int rr = r & (PT_M - 1);
+                    const uint32_t at = sb + Lay::OFF_Q + (r / PT_M) * 2 * Lay::TILE + (d >> 6) * Lay::PANEL +
+                                        (rr >> 3) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
+                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at), "r"(*reinterpret_cast<const uint32_t *>(&h0)),
+                                 "r"(*reinterpret_cast<const uint32_t *>(&h1)) : "memory");
+                    if (q_lo)
+                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at + Lay::TILE),
+                                     "r"(half2_bits(v0 - __low2float(h0), v1 - __high2float(h0))),
+                                     "r"(half2_bits(v2 - __low2float(h1), v3 - __high2float(h1))) : "memory");
+                };
+                put(oct_a(o, neox), x.a);
+                put(oct_b(o, HD, neox), x.b);
+            }
+        }
+    }
+    fence_proxy_async();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const bool mods = a.cap > 0.0f || a.slopes != nullptr;
-    const bool q_lo = SPLIT || a.rope.half > 0;
     const uint32_t TM_S[2] = {tmem, tmem + 128}, TM_O[2] = {tmem + 256, tmem + 256 + HD};
 
     if (warp < PT_W_CONV) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        // ---- q: OL lanes per row, one eight-channel piece each, eight rows'
-        // loads in flight
-        {
-            constexpr int OL = HD / 8, RPW = 32 / OL, STEP = PT_W_CONV * RPW, U = 8;
-            const T *q = static_cast<const T *>(a.q);
-            const int o = lane % OL, neox = a.rope.neox;
-            const bool turn = 4 * o < a.rope.half;
-            for (int rb = warp * RPW + lane / OL; rb < PT_ROWS; rb += U * STEP) {
-                Raw4<T> xa[U], xb[U];
-                float4 cs[U], sn[U];
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    // rows past the last one repeat it: they are not written
-                    const int r = r0 + min(rb + i * STEP, rows - 1), t = r / group, h = head * group + r - t * group;
-                    const T *src = q + (int64_t)(s.t0 + t) * a.q_stride + (int64_t)h * HD;
-                    xa[i].load(src + oct_a(o, neox));
-                    xb[i].load(src + oct_b(o, HD, neox));
-                    int64_t p = pos0 + t;
-                    if (p >= a.rope.rows) {
-                        if (turn) atomicOr(a.status, STATUS_BAD_PLAN);
-                        p = 0;
-                    }
-                    if (turn) {
-                        cs[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.cs + p * a.rope.half + 4 * o));
-                        sn[i] = __ldg(reinterpret_cast<const float4 *>(a.rope.sn + p * a.rope.half + 4 * o));
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int r = rb + i * STEP;
-                    Oct x;
-                    xa[i].get(x.a);
-                    xb[i].get(x.b);
-                    if (turn) rope_oct(x, cs[i], sn[i], neox);
-                    float m = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
-#pragma unroll
-                    for (int d = 1; d < OL; d <<= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, d));
-                    // the row's largest magnitude to [1, 2) by a power of two
-                    const int e2 = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
-                    const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-                    if (o == 0)
-                        rsv[r] = __uint_as_float((uint32_t)(127 + e2) << 23) *
-                                 (float)((double)a.scale * (mods ? 1.0 : 1.4426950408889634));
-                    auto put = [&](int d, const float (&v)[4]) {
-                        const float v0 = v[0] * inv, v1 = v[1] * inv, v2 = v[2] * inv, v3 = v[3] * inv;
-                        const uint32_t h0 = half2_bits(v0, v1), h1 = half2_bits(v2, v3);
-                        const int rr = r & (PT_M - 1);
-                        const uint32_t at = sb + Lay::OFF_Q + (r / PT_M) * 2 * Lay::TILE + (d >> 6) * Lay::PANEL +
-                                            (rr >> 3) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
-                        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at), "r"(h0), "r"(h1) : "memory");
-                        if (q_lo)
-                            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" :: "r"(at + Lay::TILE),
-                                         "r"(half2_bits(v0 - h2f(h0 & 0xffffu), v1 - h2f(h0 >> 16))),
-                                         "r"(half2_bits(v2 - h2f(h1 & 0xffffu), v3 - h2f(h1 >> 16))) : "memory");
-                    };
-                    put(oct_a(o, neox), x.a);
-                    put(oct_b(o, HD, neox), x.b);
-                }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_Q));
-            // the score factors are read by other warps
-            asm volatile("bar.sync 1, %0;" :: "n"(PT_W_CONV * 32) : "memory");
-        }
         // ---- weights: thread = row
         const int t = warp >> 2, wq = warp & 3, r = t * PT_M + wq * 32 + lane;
         const uint32_t lanes = (uint32_t)(32 * wq) << 16;
@@ -610,48 +652,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp < PT_W_MMA) {
         // ---- codes to f16, and the tiles' scales
-        constexpr int N = (Piece<HD>::COUNT + PT_NCONV - 1) / PT_NCONV;
-        const int w = warp - PT_W_CONV;
+        constexpr int N = NP;
+        const int w = cw;
         auto block_of = [&](int b) { return kv8_block(c, kv8_page(c, a, seq, b), head, b & (c.page / KV8_BLOCK - 1)); };
-        uint4 piece[N];
-        // of the tile being fetched: lane i < 8 its block i (-1 past the span);
-        // of the one after it: the page id, read a tile ahead so that no fetch
-        // waits for the table
-        int64_t blk = -1;
-        int page = -1;
-        float ksc = 0.0f, vsc = 0.0f;
-        auto find_page = [&](int j) {
-            const int b = b0 + j * PT_BLOCKS + lane;
-            page = lane < PT_BLOCKS && b < b1 ? __ldg(a.table + (int64_t)seq * a.max_pages + (b >> (c.page_shift - 4))) : -1;
-        };
-        auto find_blocks = [&](int j) {
-            const int b = b0 + j * PT_BLOCKS + lane;
-            blk = -1;
-            if (lane < PT_BLOCKS && b < b1) {
-                if ((unsigned)page >= (unsigned)c.n_pages) {
-                    atomicOr(a.status, STATUS_BAD_PLAN);
-                    page = 0;
-                }
-                blk = kv8_block(c, page, head, b & (c.page / KV8_BLOCK - 1));
-            }
-            find_page(j + 1);
-        };
-        auto fetch = [&](const int8_t *codes) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int u = w + PT_NCONV * i;
-                const int64_t mine = __shfl_sync(ALL, blk, min(u, Piece<HD>::COUNT - 1) * Piece<HD>::ROWS / KV8_BLOCK);
-                if (u < Piece<HD>::COUNT) piece[i] = piece_load<HD>(codes, mine, u, lane);
-            }
-        };
-        auto fetch_scales = [&]() {
-            ksc = w == 0 && blk >= 0 ? __ldg(c.ks + blk) : 0.0f;
-            vsc = w == 0 && blk >= 0 ? __ldg(c.vs + blk) : 0.0f;
-        };
-        find_page(0);
-        find_blocks(0);
-        fetch(c.k);
-        fetch_scales();
         // the span's largest V scale: the unit of the accumulator
         float vref = 0.0f;
         for (int b = b0 + w * 32 + lane; b < b1; b += PT_NCONV * 32) vref = fmaxf(vref, __ldg(c.vs + block_of(b)));
@@ -732,7 +735,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             commit(one, bar(B_S0 + t));
             if (t == n_mt - 1) commit(one, bar(B_FREE + x_buf(2 * j)));
         };
-        bool ok = wait(B_Q, 0) && full(0);
+        bool ok = full(0);
         if (ok) {
             tc_fence_after();
             for (int t = 0; t < n_mt; ++t) scores(t, 0);
@@ -789,11 +792,14 @@ int launch_typed(const PtParams &p, unsigned ctas, cudaStream_t st) {
 
 bool kv8_prompt_supported(int hd) { return hd == 64 || hd == 128; }
 
-int launch_kv8_prompt(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int skip_rows, cudaStream_t st) {
-    PtParams p{c, a, skip_rows};
-    // at most one partly filled tile per request
+int launch_kv8_prompt(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int skip_rows, int num_sms, cudaStream_t st) {
+    // Two tiles per CTA share its K and V and overlap one's products with the
+    // other's weights; where 256-row CTAs would not fill the GPU, one each.
     const int64_t rows = (int64_t)a.n_tok * (a.n_head / c.hkv);
-    const int64_t ctas = (rows / PT_ROWS + a.n_seq) * c.hkv;
+    const int tile_rows = rows / PT_ROWS * c.hkv >= num_sms ? PT_ROWS : PT_M;
+    PtParams p{c, a, skip_rows, tile_rows};
+    // at most one partly filled tile per request
+    const int64_t ctas = (rows / tile_rows + a.n_seq) * c.hkv;
     if (ctas > INT32_MAX) return -1;
     switch (c.hd) {
         case 64: return f16 ? launch_typed<__half, 64>(p, (unsigned)ctas, st) : launch_typed<float, 64>(p, (unsigned)ctas, st);

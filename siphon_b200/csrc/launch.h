@@ -267,7 +267,7 @@ size_t kv8_attn_workspace(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int nu
 // requests of more than skip_rows rows (query heads of a KV head x new tokens),
 // on the tensor-memory kernel; -3: head size without one
 bool kv8_prompt_supported(int hd);
-int launch_kv8_prompt(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int skip_rows, cudaStream_t st);
+int launch_kv8_prompt(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, int skip_rows, int num_sms, cudaStream_t st);
 int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *ws, int num_sms, cudaStream_t st);
 
 }  // namespace sicu
