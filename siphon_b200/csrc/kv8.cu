@@ -216,101 +216,149 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_release_kernel(const int32_t
 // A block's scale is the largest |x| it was given over 127; code = rne(x /
 // scale). Rows appended to a block that already holds some may need a larger
 // scale: the codes in place are then requantized to it (rne(code * old / new)),
-// each at most once per doubling of the scale in practice. One warp owns one
-// (block, KV head, K or V): it loads the block's new rows once into registers,
-// rotates K, reduces the magnitude, and writes codes, so a step reads its
-// inputs once and writes one byte per element; nothing is shared between warps
-// and the result does not depend on their order. Bound by DRAM bytes for
-// prompts and by one load-reduce-store latency for single tokens.
+// each at most once per doubling of the scale in practice. Two warps own one
+// (block, KV head, K or V): they load the block's new rows once into registers
+// (eight rows each), rotate K, reduce the magnitude, and write codes, so a step
+// reads its inputs once and writes one byte per element; nothing else is shared
+// and the result does not depend on any order. The slots and positions a CTA
+// needs are read at once at its start, and a row's table entries with its
+// values: two memory latencies per block, where one warp per block and its
+// reads in the order of use took four and half the warps (59 -> 49 us for 15,900
+// tokens of 8 heads of 128, f32, 165 MB). Bound by DRAM bytes for prompts and by
+// those latencies for single tokens.
 constexpr int STORE_WARPS = 4;
 // smallest magnitude worth a scale: below it 1 / scale would leave f32's range
 constexpr float KV8_TINY = 1.92592994e-34f;     // 2^-112
 
+// four codes rne(x * inv), |x * inv| <= 127: adding 1.5 2^23 leaves the rounded
+// integer in the sum's low bits
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], float inv) {
+    uint32_t q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = __float_as_uint(__fadd_rn(__fmul_rn(x[e], inv), 12582912.0f));
+    return prmt(prmt(q[0], q[1], 0x0040), prmt(q[2], q[3], 0x0040), 0x5410);
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(STORE_WARPS * 32) kv8_store_kernel(Kv8Dev c, const T *k, const T *v, int64_t k_stride,
+__global__ void __launch_bounds__(STORE_WARPS * 32, HD <= 128 ? 5 : 3) kv8_store_kernel(Kv8Dev c, const T *k, const T *v, int64_t k_stride,
                                                                      int64_t v_stride, const int64_t *slot,
                                                                      const int32_t *pos, RopeDev rope, int64_t n_tok,
                                                                      int chunk, int *status) {
     constexpr int OCTS = HD / 8;                 // 8-channel pieces per row
-    constexpr int IT = KV8_BLOCK * OCTS / 32;    // pieces per lane
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+    constexpr int ROWS = KV8_BLOCK / 2;          // rows per warp
+    constexpr int IT = ROWS * OCTS / 32;         // pieces per lane
+    __shared__ float top[2][STORE_WARPS];        // magnitudes, by job parity
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pair = warp >> 1, half = warp & 1, head = blockIdx.y;
     const int64_t c0 = (int64_t)blockIdx.x * chunk;
-    // tokens of the chunk that open a run of rows for one block
+    // tokens c0 + lane and, for runs that pass the chunk's end, c0 + 32 + lane
     const int64_t t = c0 + lane;
-    bool opens = false;
-    if (lane < chunk && t < n_tok) {
-        const int64_t s = slot[t];
-        if (s >= 0) opens = t == 0 || slot[t - 1] < 0 || (slot[t - 1] >> 4) != (s >> 4);
+    const int64_t sa = t < n_tok ? slot[t] : -1, sb = t + 32 < n_tok ? slot[t + 32] : -1;
+    const int64_t sp = lane == 0 && c0 > 0 && c0 < n_tok ? slot[c0 - 1] : -1;
+    int pa = 0, pb = 0;
+    if (rope.half) {
+        pa = t < n_tok ? pos[t] : 0;
+        pb = t + 32 < n_tok ? pos[t + 32] : 0;
     }
+    // tokens of the chunk that open a run of rows for one block
+    int64_t prev = __shfl_up_sync(0xffffffffu, sa, 1);
+    if (lane == 0) prev = sp;
+    const bool opens = lane < chunk && sa >= 0 && (prev < 0 || (prev >> 4) != (sa >> 4));
     const uint32_t starts = __ballot_sync(0xffffffffu, opens);
     const int jobs = 2 * __popc(starts);
-    for (int j = warp; j < jobs; j += STORE_WARPS) {
+    int parity = 0;
+    for (int j = pair; j < jobs; j += STORE_WARPS / 2, parity ^= 1) {
         const bool is_v = j & 1;
-        const int64_t r0 = c0 + __fns(starts, 0, (j >> 1) + 1);
-        // the run: rows r0 .. r0 + n - 1 in one block
-        int64_t s = -1;
-        if (lane < KV8_BLOCK && r0 + lane < n_tok) s = slot[r0 + lane];
+        const int i0 = __fns(starts, 0, (j >> 1) + 1);
+        const int64_t r0 = c0 + i0;
+        // the run: rows r0 .. r0 + n - 1 in one block; lane i knows row i
+        const int from = i0 + lane;
+        const int64_t s1 = __shfl_sync(0xffffffffu, sa, from & 31), s2 = __shfl_sync(0xffffffffu, sb, from & 31);
+        const int q1 = __shfl_sync(0xffffffffu, pa, from & 31), q2 = __shfl_sync(0xffffffffu, pb, from & 31);
+        const int64_t s = from < 32 ? s1 : s2;
         const int64_t s0 = __shfl_sync(0xffffffffu, s, 0);
-        const uint32_t same = __ballot_sync(0xffffffffu, s >= 0 && (s >> 4) == (s0 >> 4));
+        const uint32_t same = __ballot_sync(0xffffffffu, lane < KV8_BLOCK && s >= 0 && (s >> 4) == (s0 >> 4));
         const int n = __ffs(~same) - 1;
         const int off = (int)(s & (KV8_BLOCK - 1)), lead = __shfl_sync(0xffffffffu, off, 0);
-        const int64_t pg = s0 >> c.page_shift;
-        if (pg >= c.n_pages) {
-            if (lane == 0) atomicOr(status, STATUS_BAD_PLAN);
-            continue;
+        int p = from < 32 ? q1 : q2;
+        if (rope.half && lane < n && (p < 0 || p >= rope.rows)) {
+            atomicOr(status, STATUS_BAD_PLAN);
+            p = -1;
         }
-        const int64_t blk = kv8_block(c, (int)pg, head, (int)(s0 & (c.page - 1)) >> 4);
-        const T *src = (is_v ? v : k) + r0 * (is_v ? v_stride : k_stride) + (int64_t)head * HD;
+        const int64_t pg = s0 >> c.page_shift;
+        const bool in = pg < c.n_pages;
+        if (!in && lane == 0) atomicOr(status, STATUS_BAD_PLAN);
+        const int64_t blk = in ? kv8_block(c, (int)pg, head, (int)(s0 & (c.page - 1)) >> 4) : 0;
         const int64_t stride = is_v ? v_stride : k_stride;
+        const T *src = (is_v ? v : k) + r0 * stride + (int64_t)head * HD;
         const int neox = is_v ? 0 : rope.neox;
         float *scale = (is_v ? c.vs : c.ks) + blk;
         int8_t *codes = (is_v ? c.v : c.k) + blk * (KV8_BLOCK * HD);
-        const float before = lead > 0 ? *scale : 0.0f;
-        Oct x[IT];
-        float amax = 0.0f;
-        bool odd = false;
+        const float before = in && lead > 0 ? *scale : 0.0f;
+        Raw4<T> xa[IT], xb[IT];
+        float4 cs[IT], sn[IT];
+        const bool turn = !is_v && rope.half;
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
-            if (row < n) {
-                load4(src + row * stride + oct_a(o, neox), x[it].a);
-                load4(src + row * stride + oct_b(o, HD, neox), x[it].b);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[it].a[e] = x[it].b[e] = 0.0f;
+            const int idx = it * 32 + lane, row = half * ROWS + idx / OCTS, o = idx % OCTS;
+            const int pr = __shfl_sync(0xffffffffu, p, row);
+            // rows past the run repeat its last one and are not written
+            const T *sr = src + min(row, n - 1) * stride;
+            xa[it].load(sr + oct_a(o, neox));
+            xb[it].load(sr + oct_b(o, HD, neox));
+            if (turn && 4 * o < rope.half) {
+                const int64_t at = (int64_t)max(row < n ? pr : 0, 0) * rope.half + 4 * o;
+                cs[it] = __ldg(reinterpret_cast<const float4 *>(rope.cs + at));
+                sn[it] = __ldg(reinterpret_cast<const float4 *>(rope.sn + at));
             }
         }
-        if (!is_v && rope.half) {
+        Oct x[IT];
+        float amax = 0.0f, zero = 0.0f;
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
-                if (row < n) {
-                    const int64_t p = pos[r0 + row];
-                    if (p >= 0 && p < rope.rows) rope_oct(x[it], rope, p, o);
-                    else if (o == 0) atomicOr(status, STATUS_BAD_PLAN);
+        for (int it = 0; it < IT; ++it) {
+            const int idx = it * 32 + lane, row = half * ROWS + idx / OCTS, o = idx % OCTS;
+            const int pr = __shfl_sync(0xffffffffu, p, row);
+            xa[it].get(x[it].a);
+            xb[it].get(x[it].b);
+            if (turn && 4 * o < rope.half && pr >= 0) rope_oct(x[it], cs[it], sn[it], neox);
+            if (row < n) {
+                // 0 x is NaN where x is not finite
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    amax = fmaxf(amax, fmaxf(fabsf(x[it].a[e]), fabsf(x[it].b[e])));
+                    zero = fmaf(x[it].a[e], 0.0f, fmaf(x[it].b[e], 0.0f, zero));
                 }
             }
         }
+        const bool odd = __any_sync(0xffffffffu, zero != 0.0f);
+        if (odd) {
+            // the largest finite magnitude
+            amax = 0.0f;
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
+            for (int it = 0; it < IT; ++it) {
+                if (half * ROWS + (it * 32 + lane) / OCTS < n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float ma = fabsf(x[it].a[e]), mb = fabsf(x[it].b[e]);
-                const bool fa = ma <= 3.402823466e38f, fb = mb <= 3.402823466e38f;
-                odd |= !fa || !fb;
-                amax = fmaxf(amax, fmaxf(fa ? ma : 0.0f, fb ? mb : 0.0f));
+                    for (int e = 0; e < 4; ++e) {
+                        const float ma = fabsf(x[it].a[e]), mb = fabsf(x[it].b[e]);
+                        amax = fmaxf(amax, fmaxf(ma < INFINITY ? ma : 0.0f, mb < INFINITY ? mb : 0.0f));
+                    }
+                }
             }
+            if (lane == 0) atomicOr(status, STATUS_NONFINITE);
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        if (lane == 0) top[parity][warp] = amax;
+        // both warps of the pair have read the scale, and see each other's rows
+        asm volatile("bar.sync %0, 64;" :: "r"(1 + pair) : "memory");
+        amax = fmaxf(amax, top[parity][warp ^ 1]);
+        if (!in) continue;
         const float sc = fmaxf(before, amax >= KV8_TINY ? __fdiv_rn(amax, 127.0f) : 0.0f);
         const float inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
-        if (__any_sync(0xffffffffu, odd) && lane == 0) atomicOr(status, STATUS_NONFINITE);
         if (sc > before && lead > 0) {
             // rows stored earlier: their codes at the larger scale
             const float r = __fmul_rn(before, inv);
             uint32_t *w = reinterpret_cast<uint32_t *>(codes);
-            for (int i = lane; i < lead * (HD / 4); i += 32) {
+            for (int i = lane + 32 * half; i < lead * (HD / 4); i += 64) {
                 const uint32_t u = w[i];
                 uint32_t o = 0;
 #pragma unroll
@@ -321,21 +369,26 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) kv8_store_kernel(Kv8Dev c, c
                 w[i] = o;
             }
         }
-        if (lane == 0) *scale = sc;
+        if (lane == 0 && half == 0) *scale = sc;
 #pragma unroll
         for (int it = 0; it < IT; ++it) {
-            const int idx = it * 32 + lane, row = idx / OCTS, o = idx % OCTS;
-            // one row per lane below: the row's own offset in its block
-            const int at = __shfl_sync(0xffffffffu, off, row);
+            const int idx = it * 32 + lane, row = half * ROWS + idx / OCTS, o = idx % OCTS;
+            const int at = __shfl_sync(0xffffffffu, off, row);       // the row's place in its block
             if (row < n) {
-                uint32_t wa = 0, wb = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                uint32_t wa, wb;
+                if (odd) {
                     // a NaN becomes 0, an infinity the largest code of its sign
-                    const int qa = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].a[e], inv))));
-                    const int qb = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].b[e], inv))));
-                    wa |= ((uint32_t)qa & 0xffu) << (8 * e);
-                    wb |= ((uint32_t)qb & 0xffu) << (8 * e);
+                    wa = wb = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int qa = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].a[e], inv))));
+                        const int qb = min(127, max(-127, __float2int_rn(__fmul_rn(x[it].b[e], inv))));
+                        wa |= ((uint32_t)qa & 0xffu) << (8 * e);
+                        wb |= ((uint32_t)qb & 0xffu) << (8 * e);
+                    }
+                } else {
+                    wa = codes4(x[it].a, inv);
+                    wb = codes4(x[it].b, inv);
                 }
                 int8_t *dst = codes + at * HD;
                 if (neox) {
@@ -350,34 +403,39 @@ __global__ void __launch_bounds__(STORE_WARPS * 32) kv8_store_kernel(Kv8Dev c, c
 }
 
 // ---- load ----------------------------------------------------------------------------
-// Rows of the cache as values: code * scale. 16 codes per thread; bound by the
-// bytes of the values written.
+// Rows of the cache as values: code * scale. A CTA takes eight rows; a lane four
+// codes at a time, so that a warp writes 512 consecutive bytes (16 codes per
+// lane, four strided stores, wrote half sectors: 41 us against 33 for 15,900
+// rows of 8 heads of 128, f32, 163 MB), K's and V's read before either is written.
+// Bound by the bytes of the values written.
+constexpr int LOAD_ROWS = 8;
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_load_kernel(Kv8Dev c, const int64_t *slot, int64_t n_tok, T *k, T *v,
                                                        int *status) {
-    const int pieces = c.hkv * c.hd / 16, per_head = c.hd / 16;
-    const bool is_v = blockIdx.y;
-    const int64_t total = n_tok * pieces;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = i / pieces;
-        const int p = (int)(i - t * pieces), head = p / per_head, e = p - head * per_head;
-        const int64_t s = slot[t], pg = s >> c.page_shift;
-        T *dst = (is_v ? v : k) + (t * c.hkv + head) * c.hd + e * 16;
-        if (s < 0 || pg >= c.n_pages) {
-            if (s >= 0) atomicOr(status, STATUS_BAD_PLAN);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) store4(dst + 4 * j, 0.0f, 0.0f, 0.0f, 0.0f);
-            continue;
+    const unsigned per_head = c.hd / 4, words = c.hkv * per_head;
+    const int64_t t0 = (int64_t)blockIdx.x * LOAD_ROWS;
+    const unsigned rows = (unsigned)(n_tok - t0 < LOAD_ROWS ? n_tok - t0 : LOAD_ROWS);
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < rows * words; i += 256) {
+        const unsigned r = i / words, p = i - r * words, head = p / per_head, e = p - head * per_head;
+        const int64_t s = __ldg(slot + t0 + r), pg = s >> c.page_shift;
+        const int64_t dst = ((t0 + r) * c.hkv + head) * c.hd + e * 4;
+        uint32_t wk = 0, wv = 0;
+        float sk = 0.0f, sv = 0.0f;
+        if (s >= 0 && pg < c.n_pages) {
+            const int64_t blk = kv8_block(c, (int)pg, head, (int)(s & (c.page - 1)) >> 4);
+            const int64_t at = (blk * KV8_BLOCK + (s & (KV8_BLOCK - 1))) * c.hd + e * 4;
+            wk = *reinterpret_cast<const uint32_t *>(c.k + at);
+            wv = *reinterpret_cast<const uint32_t *>(c.v + at);
+            sk = c.ks[blk];
+            sv = c.vs[blk];
+        } else if (s >= 0) {
+            atomicOr(status, STATUS_BAD_PLAN);
         }
-        const int64_t blk = kv8_block(c, (int)pg, head, (int)(s & (c.page - 1)) >> 4);
-        const float sc = (is_v ? c.vs : c.ks)[blk];
-        const int8_t *src = (is_v ? c.v : c.k) + (blk * KV8_BLOCK + (s & (KV8_BLOCK - 1))) * c.hd + e * 16;
-        const uint4 w = *reinterpret_cast<const uint4 *>(src);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            store4(dst + 4 * j, (float)(int8_t)u[j] * sc, (float)(int8_t)(u[j] >> 8) * sc,
-                   (float)(int8_t)(u[j] >> 16) * sc, (float)(int8_t)(u[j] >> 24) * sc);
+        store4(k + dst, (float)(int8_t)wk * sk, (float)(int8_t)(wk >> 8) * sk, (float)(int8_t)(wk >> 16) * sk,
+               (float)(int8_t)(wk >> 24) * sk);
+        store4(v + dst, (float)(int8_t)wv * sv, (float)(int8_t)(wv >> 8) * sv, (float)(int8_t)(wv >> 16) * sv,
+               (float)(int8_t)(wv >> 24) * sv);
     }
 }
 
@@ -416,9 +474,11 @@ int launch_kv8_plan(const Kv8PlanLaunch &L, cudaStream_t st) {
     // barrier cost more than they share out), eight for steps with prompts.
     const int ctas = L.max_tok > 4 * PLAN_THREADS ? 8 : 1;
     const size_t smem = (size_t)(3 * L.n_seq + 2) * 4;
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kv8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return -2;
+    if (smem > 48 * 1024 && !allow_smem<&kv8_plan_kernel>((3 * KV8_MAX_SEQ + 2) * 4)) return -2;
+    if (ctas == 1) {
+        kv8_plan_kernel<<<1, PLAN_THREADS, smem, st>>>(L);
+        return cudaGetLastError() == cudaSuccess ? 0 : -2;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(PLAN_THREADS);
@@ -450,9 +510,7 @@ int launch_kv8_store(const Kv8Dev &c, bool f16, const void *k, const void *v, in
 
 int launch_kv8_load(const Kv8Dev &c, bool f16, const int64_t *slot, int64_t n_tok, void *k, void *v, int *status,
                     cudaStream_t st) {
-    const int64_t items = n_tok * (c.hkv * c.hd / 16);
-    const int64_t ctas = (items + 255) / 256;
-    const dim3 grid((unsigned)(ctas < (1 << 20) ? ctas : (1 << 20)), 2);
+    const unsigned grid = (unsigned)((n_tok + LOAD_ROWS - 1) / LOAD_ROWS);
     if (f16)
         kv8_load_kernel<__half><<<grid, 256, 0, st>>>(c, slot, n_tok, static_cast<__half *>(k), static_cast<__half *>(v), status);
     else

@@ -605,8 +605,7 @@ template <typename T, int HD, int NT>
 int launch_typed(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
     const dim3 grid((unsigned)(g.row_tiles * c.hkv), (unsigned)g.splits, (unsigned)a.n_seq);
     constexpr int smem = AttnCfg<T, HD, NT>::SMEM;
-    if (cudaFuncSetAttribute(kv8_attn_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return -2;
+    if (!allow_smem<&kv8_attn_kernel<T, HD, NT>>(smem)) return -2;
     kv8_attn_kernel<T, HD, NT><<<grid, AT_WARPS * 32, smem, st>>>(c, a, g, ws);
     if (cudaGetLastError() != cudaSuccess) return -2;
     if (g.splits > 1) {

@@ -782,8 +782,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
 template <typename T, int HD>
 int launch_typed(const PtParams &p, unsigned ctas, cudaStream_t st) {
     constexpr int smem = PtLay<HD>::SMEM;
-    if (cudaFuncSetAttribute(kv8_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return -2;
+    if (!allow_smem<&kv8_prompt_kernel<T, HD>>(smem)) return -2;
     kv8_prompt_kernel<T, HD><<<ctas, PT_THREADS, smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

@@ -2,6 +2,7 @@
 // C ABI (abi.cu). Return 0 on success, negative on a launch problem.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -208,7 +209,22 @@ int launch_dequant(uint32_t wtype, const void *w, int64_t n_in, const int64_t *r
 // greedy choice (first maximum) of m rows of n floats into out[m]
 int launch_argmax(const float *x, int64_t n, int64_t m, int64_t *out, cudaStream_t st);
 
-// ---- paged 8-bit KV cache (kv8.cu, kv8_attn.cu) ----
+// Allows kernel f `bytes` of dynamic shared memory, once per device and
+// instantiation of this function (the attribute lives as long as the process;
+// setting it again on every launch would cost a decode step a microsecond).
+template <auto f>
+inline bool allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return true;
+    if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
+}
+
+// ---- paged 8-bit KV cache (kv8.cu, kv8_attn.cu, kv8_prompt.cu) ----
 constexpr int KV8_BLOCK = 16;         // tokens that share a scale
 constexpr int KV8_MAX_SEQ = 8192;     // requests per step
 struct Kv8Dev {
