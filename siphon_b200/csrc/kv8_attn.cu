@@ -5,17 +5,19 @@
 //   out_r = sum_j 2^(z_rj - m_r) v_j / sum_j 2^(z_rj - m_r)   over visible j
 //
 // The rows of one KV head (its n_head / n_head_kv query heads times a
-// request's new tokens) are the N side of m16n8k16 products, the cache the M
-// side: a warp takes 16 keys (one quantization block: one scale each for K
-// and V) at a time from its own ring of bulk copies, loads the codes in an order
-// of channels and keys that makes every register an operand fragment after
-// byte -> f16 expansion (|code| <= 127 is exact in f16), forms S^T = K Q^T,
-// the weights in f32, and accumulates O^T += V^T P^T. Sums, maxima and the
-// output stay in f32.
-//
-// The rotated q enters as two f16 parts (hi + lo, 22 bits), so scores agree
-// with an f32 computation. So do f32 callers' weights; f16 callers' weights
-// are rounded once to f16 (2^-11, the size of the output's own rounding).
+// request's new tokens) are the N side of the products, the cache the M side:
+// a warp takes 16 keys (one quantization block: one scale each for K and V) at
+// a time from its own ring of bulk copies, and loads the codes in an order of
+// channels and keys that makes every register an operand fragment.
+//   S^T = K Q^T        s8 MMAs (m16n8k32) on K's codes as they are; q as
+//                      integers of 24 bits in three s8 digits, exact sums
+//   O^T += V^T P^T     f16 MMAs (m16n8k16): V's codes expanded byte -> f16
+//                      (|code| <= 127 is exact there), the weights as two f16
+//                      parts (hi + lo, 22 bits) for f32 callers, rounded once
+//                      to f16 (2^-11, the size of the output's own rounding)
+//                      for f16 callers
+// Maxima, sums and the output stay in f32. Bound by issue: expanding V and the
+// weights cost about as many instructions as DRAM gives time for at its rate.
 #include "kv8.cuh"
 #include "tc.cuh"
 
@@ -29,16 +31,21 @@ constexpr int AT_MOST = 32;
 // by 2^8: weights stay below 2^8 and f16 carries them as precisely.
 constexpr float AT_LAZY = 8.0f;
 constexpr float LOWEST = -3.402823466e38f;
+constexpr float Q_TOP = 8323072.0f;       // 127 2^16, the largest of q's integers
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
 // two codes biased by 128 (bytes i, j of x) as exact halves: 0x6400 | u is 1024 + u
@@ -118,10 +125,12 @@ struct AttnCfg {
     static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
     static constexpr int OUT = AT_WARPS * R * HD * 4;                    // the warps' accumulators, after the ring's last use
     static constexpr int MAIN = RING > OUT ? RING : OUT;
-    static constexpr int QROW = R * HD * 4;                              // rotated q
-    static constexpr bool Q_REGS = NT == 1 && HD <= 128;                 // q's fragments in registers, or here:
-    static constexpr int QF = Q_REGS ? 0 : KW * NT * 2 * 32 * 8;         // [word][n tile][hi, lo][lane]
-    static constexpr int SMEM = MAIN + QROW + QF;
+    static constexpr int QROW = R * HD * 4;                              // rotated q, then its fragments:
+    static constexpr int QF = KW * NT * 32 * 16;                         // [word][n tile][lane] three digits
+    static constexpr bool Q_REGS = NT == 1 && HD <= 128;                 // kept in registers
+    static constexpr int SMEM = MAIN + QROW;
+    static constexpr bool V_EARLY = NT == 1 && HD <= 128;
+    static_assert(QF <= QROW, "fragments over the rows");
 };
 
 template <typename T, int HD, int NT>
@@ -134,8 +143,8 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     constexpr int PARTS = SPLIT ? 2 : 1;        // of the weights
     extern __shared__ __align__(128) uint8_t at_sm[];
     float *qrow = reinterpret_cast<float *>(at_sm + Cfg::MAIN);
-    uint2 *qf = reinterpret_cast<uint2 *>(at_sm + Cfg::MAIN + Cfg::QROW);
-    __shared__ float rscale[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
+    uint4 *qf = reinterpret_cast<uint4 *>(qrow);
+    __shared__ float rscale[R], qinv[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
     __shared__ int row_lo[R], row_hi[R], row_pos[R];
     __shared__ float row_slope[R];
     __shared__ __align__(8) uint64_t bars[AT_WARPS * AT_STAGES];
@@ -202,18 +211,24 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         store4(qrow + r * HD + oct_b(o, HD, neox), x.b[0], x.b[1], x.b[2], x.b[3]);
     }
     __syncthreads();
-    // A row's largest magnitude is brought to [1, 2) by a power of two, so
-    // that its f16 parts neither overflow nor lose small rows; the factor
-    // goes back in with the score's scale.
+    // A row becomes 24-bit integers of its largest magnitude / (127 2^16), in
+    // three signed base-256 digits: products with the codes are then exact s8
+    // MMAs on the codes as they are, and a score is as good as from f32 q.
     for (int r = warp; r < R; r += AT_WARPS) {
-        float m = 0.0f;
-        for (int d = lane; d < HD; d += 32) m = fmaxf(m, fabsf(qrow[r * HD + d]));
+        float m = 0.0f, zero = 0.0f;
+        for (int d = lane; d < HD; d += 32) {
+            m = fmaxf(m, fabsf(qrow[r * HD + d]));
+            zero = fmaf(qrow[r * HD + d], 0.0f, zero);        // NaN unless all are finite
+        }
 #pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        for (int d = 16; d; d >>= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            zero += __shfl_xor_sync(0xffffffffu, zero, d);
+        }
         if (lane == 0) {
-            // exponent of the magnitude, kept where both factors are normal
-            const int e = min(max((int)((__float_as_uint(m) >> 23) & 255) - 127, -100), 100);
-            rscale[r] = __uint_as_float((uint32_t)(127 + e) << 23);
+            m = fmaxf(m, 1e-30f);                             // smaller rows count as zero
+            qinv[r] = __fdiv_rn(Q_TOP, m);
+            rscale[r] = __fdiv_rn(m, Q_TOP) + zero;
             if (r < rows) {
                 const int t = (rt * R + r) / group, p = s.len - s.n_new + t;
                 row_pos[r] = p;
@@ -227,26 +242,42 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         }
     }
     __syncthreads();
-    // the fragment words of q row nt * 8 + (ln >> 2) for k-step w
-    auto q_frag = [&](int w, int nt, int ln, uint2 &hi, uint2 &lo) {
-        const int r = nt * 8 + (ln >> 2), d = (w / WPC) * (16 * WPC) + (ln & 3) * (4 * WPC) + (w % WPC) * 4;
-        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(rscale[r]));     // 1 / a power of two
-        const float4 f = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
-        const float x0 = f.x * inv, x1 = f.y * inv, x2 = f.z * inv, x3 = f.w * inv;
-        hi = make_uint2(half2_bits(x0, x1), half2_bits(x2, x3));
-        lo = make_uint2(half2_bits(x0 - h2f(hi.x & 0xffffu), x1 - h2f(hi.x >> 16)),
-                        half2_bits(x2 - h2f(hi.y & 0xffffu), x3 - h2f(hi.y >> 16)));
-    };
-    uint2 qreg[Cfg::Q_REGS ? KW : 1][2];
-    if constexpr (Cfg::Q_REGS) {
+    // fragment word w of q row nt * 8 + (ln >> 2): its digits of four channels,
+    // formed once per CTA and put over the rows
+    {
+        constexpr int WORDS = KW * NT * 32, N = (WORDS + AT_WARPS * 32 - 1) / (AT_WARPS * 32);
+        uint4 word[N];
 #pragma unroll
-        for (int w = 0; w < KW; ++w) q_frag(w, 0, lane, qreg[w][0], qreg[w][1]);
-    } else {
-        for (int i = tid; i < KW * NT * 32; i += AT_WARPS * 32) {
-            const int ln = i & 31, nt = (i >> 5) % NT, w = i / (32 * NT);
-            q_frag(w, nt, ln, qf[((w * NT + nt) * 2) * 32 + ln], qf[((w * NT + nt) * 2 + 1) * 32 + ln]);
+        for (int k = 0; k < N; ++k) {
+            const int i = min(tid + k * AT_WARPS * 32, WORDS - 1), ln = i & 31, nt = (i >> 5) % NT, w = i / (32 * NT);
+            const int r = nt * 8 + (ln >> 2), d = (w / WPC) * (16 * WPC) + (ln & 3) * (4 * WPC) + (w % WPC) * 4;
+            const float inv = qinv[r];
+            const float4 f = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
+            const int q0 = __float2int_rn(f.x * inv), q1 = __float2int_rn(f.y * inv), q2 = __float2int_rn(f.z * inv),
+                      q3 = __float2int_rn(f.w * inv);
+            // digits of x: its bytes, each carrying into the next where the
+            // lower one counts as negative
+            const int a0 = q0 + 0x8080, a1 = q1 + 0x8080, a2 = q2 + 0x8080, a3 = q3 + 0x8080;
+            const uint32_t l01 = prmt(a0, a1, 0x5140), l23 = prmt(a2, a3, 0x5140);       // bytes 0, 0, 1, 1
+            const uint32_t h01 = prmt(a0, a1, 0x0062), h23 = prmt(a2, a3, 0x0062);       // bytes 2, 2
+            word[k] = make_uint4(prmt(h01, h23, 0x5410), prmt(l01, l23, 0x7632) ^ 0x80808080u,
+                                 prmt(l01, l23, 0x5410) ^ 0x80808080u, 0);
         }
         __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (tid + k * AT_WARPS * 32 < WORDS) qf[tid + k * AT_WARPS * 32] = word[k];
+    }
+    __syncthreads();
+    uint32_t qreg[Cfg::Q_REGS ? KW : 1][3];
+    if constexpr (Cfg::Q_REGS) {
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const uint4 f = qf[w * 32 + lane];
+            qreg[w][0] = f.x;
+            qreg[w][1] = f.y;
+            qreg[w][2] = f.z;
+        }
     }
 
     // ---- keys
@@ -290,45 +321,64 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         const uint32_t kbuf = ring + st * Cfg::STAGE, vbuf = kbuf + KV8_BLOCK * HD;
         const int b = b0 + i;
         const float kscale = __shfl_sync(0xffffffffu, ks, i), vscale = __shfl_sync(0xffffffffu, vs, i);
-        // S^T: 16 keys x R rows, the parts of q in accumulators of their own
-        float z[NT][4], zl[NT][4];
+        // S^T: 16 keys x R rows, each digit of q in an accumulator of its own
+        // that starts at the bits of 1.5 2^23: the sums (below 2^22) then are
+        // the floats 1.5 2^23 + sum
+        float z[NT][4];
+        {
+            int acc[3][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int d = 0; d < 3; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[nt][e] = zl[nt][e] = 0.0f;
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int ch = 0; ch < KW / WPC; ++ch) {
-            uint32_t k0[WPC], k1[WPC];
-            lds_words<WPC>(kbuf + gq * HD + ch * (16 * WPC) + tq * (4 * WPC), k0);
-            lds_words<WPC>(kbuf + (gq + 8) * HD + ch * (16 * WPC) + tq * (4 * WPC), k1);
+                    for (int e = 0; e < 4; ++e) acc[d][nt][e] = 0x4b400000;
 #pragma unroll
-            for (int e = 0; e < WPC; ++e) {
-                const int w = ch * WPC + e;
-                const uint32_t x = k0[e] ^ 0x80808080u, y = k1[e] ^ 0x80808080u;
-                const uint32_t af[4] = {code_pair(x, 0x4140), code_pair(y, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4342)};
+            for (int ch = 0; ch < KW / WPC; ++ch) {
+                uint32_t k0[WPC], k1[WPC];
+                lds_words<WPC>(kbuf + gq * HD + ch * (16 * WPC) + tq * (4 * WPC), k0);
+                lds_words<WPC>(kbuf + (gq + 8) * HD + ch * (16 * WPC) + tq * (4 * WPC), k1);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    uint2 f, fl;
-                    if constexpr (Cfg::Q_REGS) {
-                        f = qreg[w][0];
-                        fl = qreg[w][1];
-                    } else {
-                        f = qf[((w * NT + nt) * 2) * 32 + lane];
-                        fl = qf[((w * NT + nt) * 2 + 1) * 32 + lane];
+                for (int e = 0; e < WPC; e += 2) {
+                    const int w = ch * WPC + e;
+                    const uint32_t af[4] = {k0[e], k1[e], k0[e + 1], k1[e + 1]};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if constexpr (Cfg::Q_REGS) {
+#pragma unroll
+                            for (int d = 0; d < 3; ++d) mma_s8(acc[d][nt], af, qreg[w][d], qreg[w + 1][d]);
+                        } else {
+                            const uint4 f = qf[(w * NT + nt) * 32 + lane], h = qf[((w + 1) * NT + nt) * 32 + lane];
+                            mma_s8(acc[0][nt], af, f.x, h.x);
+                            mma_s8(acc[1][nt], af, f.y, h.y);
+                            mma_s8(acc[2][nt], af, f.z, h.z);
+                        }
                     }
-                    mma_f16(z[nt], af, f.x, f.y);
-                    mma_f16(zl[nt], af, fl.x, fl.y);
                 }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f0 = __int_as_float(acc[0][nt][e]) - 12582912.0f, f1 = __int_as_float(acc[1][nt][e]) - 12582912.0f,
+                                f2 = __int_as_float(acc[2][nt][e]) - 12582912.0f;
+                    z[nt][e] = fmaf(f0, 65536.0f, fmaf(f1, 256.0f, f2));
+                }
+        }
+        // V's codes on their way to registers under the scores and weights
+        uint32_t vw[Cfg::V_EARLY ? 4 : 1][Cfg::V_EARLY ? VW : 1];
+        const uint32_t vp = vbuf + 2 * tq * HD + gq * (HD / 8);
+        if constexpr (Cfg::V_EARLY) {
+#pragma unroll
+            for (int ch = 0; ch < VW / VL; ++ch)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    lds_words<VL>(vp + ((r & 1) + 8 * (r >> 1)) * HD + ch * (4 * VL), *reinterpret_cast<uint32_t (*)[VL]>(&vw[r][ch * VL]));
         }
         const int j0 = b * KV8_BLOCK + gq;           // this thread's keys: j0 and j0 + 8
         const bool masked = (b << 4) < all_lo || (b << 4) + 16 > all_hi;
         bool grow = vscale > vref;
         // y = z - m in powers of two; hidden keys -inf
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[nt][e] += zl[nt][e];
         if (mods) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -411,17 +461,21 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         // O^T += V^T P^T: a word holds four channels, two per m tile
 #pragma unroll
         for (int ch = 0; ch < VW / VL; ++ch) {
-            uint32_t v0[VL], v1[VL], v2[VL], v3[VL];
-            const uint32_t vp = vbuf + 2 * tq * HD + gq * (HD / 8) + ch * (4 * VL);
-            lds_words<VL>(vp, v0);
-            lds_words<VL>(vp + HD, v1);
-            lds_words<VL>(vp + 8 * HD, v2);
-            lds_words<VL>(vp + 9 * HD, v3);
+            uint32_t v[4][VL];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (Cfg::V_EARLY) {
+#pragma unroll
+                    for (int e = 0; e < VL; ++e) v[r][e] = vw[r][ch * VL + e];
+                } else {
+                    lds_words<VL>(vp + ((r & 1) + 8 * (r >> 1)) * HD + ch * (4 * VL), v[r]);
+                }
+            }
 #pragma unroll
             for (int e = 0; e < VL; ++e) {
                 const int w = ch * VL + e;
-                const uint32_t p0 = v0[e] ^ 0x80808080u, p1 = v1[e] ^ 0x80808080u, p2 = v2[e] ^ 0x80808080u,
-                               p3 = v3[e] ^ 0x80808080u;
+                const uint32_t p0 = v[0][e] ^ 0x80808080u, p1 = v[1][e] ^ 0x80808080u, p2 = v[2][e] ^ 0x80808080u,
+                               p3 = v[3][e] ^ 0x80808080u;
                 const uint32_t x0 = prmt(p0, p1, 0x5140), x1 = prmt(p0, p1, 0x7362);
                 const uint32_t y0 = prmt(p2, p3, 0x5140), y1 = prmt(p2, p3, 0x7362);
                 const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
