@@ -31,7 +31,6 @@ constexpr int AT_MOST = 32;
 // by 2^8: weights stay below 2^8 and f16 carries them as precisely.
 constexpr float AT_LAZY = 8.0f;
 constexpr float LOWEST = -3.402823466e38f;
-constexpr float Q_TOP = 8323072.0f;       // 127 2^16, the largest of q's integers
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -114,40 +113,44 @@ __device__ __forceinline__ Span tile_span(const Kv8AttnDev &a, const Kv8Seq &s, 
     return r;
 }
 
-// Blocks of a warp in flight at once: enough bytes per SM for DRAM's latency
-// (three stages of 4 KB, 16 warps) with four CTAs' rings in its shared memory.
-constexpr int AT_STAGES = 3;
-
 template <typename T, int HD, int NT>
 struct AttnCfg {
     static constexpr int R = 8 * NT, KW = HD / 16, VW = HD / 32;
-    static constexpr int STAGE = 2 * KV8_BLOCK * HD;                     // K and V codes of one block
-    static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
+    // A warp's ring: two stages of two blocks, which also makes the work of an
+    // iteration two independent halves (one block and three stages with a
+    // fourth CTA per SM took 121 us against 119 for 64 requests of 4250 tokens
+    // at the Llama-3-8B shape, 42 against 34 for 48 under a window of 1024); one block where two would not leave room for CTAs.
+    static constexpr int PB = HD <= 128 ? 2 : 1, STAGES = HD <= 128 ? 2 : 3;
+    static constexpr int BLOCK = 2 * KV8_BLOCK * HD;                     // K and V codes of one block
+    static constexpr int STAGE = PB * BLOCK;
+    static constexpr int RING = AT_WARPS * STAGES * STAGE;
+    static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;                // of q's integers
+    static constexpr float Q_TOP = sizeof(T) == 4 ? 8323072.0f : 32512.0f;   // 127 256^(DIGITS - 1), the largest
     static constexpr int OUT = AT_WARPS * R * HD * 4;                    // the warps' accumulators, after the ring's last use
     static constexpr int MAIN = RING > OUT ? RING : OUT;
     static constexpr int QROW = R * HD * 4;                              // rotated q, then its fragments:
     static constexpr int QF = KW * NT * 32 * 16;                         // [word][n tile][lane] three digits
     static constexpr bool Q_REGS = NT == 1 && HD <= 128;                 // kept in registers
     static constexpr int SMEM = MAIN + QROW;
-    static constexpr bool V_EARLY = NT == 1 && HD <= 128;
     static_assert(QF <= QROW, "fragments over the rows");
 };
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(AT_WARPS * 32, HD * NT <= 128 ? 4 : HD * NT <= 256 ? 2 : 1)
+__global__ void __launch_bounds__(AT_WARPS * 32, HD * NT <= 128 ? 3 : HD * NT <= 256 ? 2 : 1)
 kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     using Cfg = AttnCfg<T, HD, NT>;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int R = Cfg::R, KW = Cfg::KW, VW = Cfg::VW, WPC = HD % 64 == 0 ? 4 : 2;
     constexpr int VL = HD % 128 == 0 ? 4 : HD % 64 == 0 ? 2 : 1;
     constexpr int PARTS = SPLIT ? 2 : 1;        // of the weights
+    constexpr int PB = Cfg::PB, STAGES = Cfg::STAGES, DIGITS = Cfg::DIGITS;
     extern __shared__ __align__(128) uint8_t at_sm[];
     float *qrow = reinterpret_cast<float *>(at_sm + Cfg::MAIN);
     uint4 *qf = reinterpret_cast<uint4 *>(qrow);
     __shared__ float rscale[R], qinv[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
     __shared__ int row_lo[R], row_hi[R], row_pos[R];
     __shared__ float row_slope[R];
-    __shared__ __align__(8) uint64_t bars[AT_WARPS * AT_STAGES];
+    __shared__ __align__(8) uint64_t bars[AT_WARPS * STAGES];
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the combine, which waits for this grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
@@ -171,22 +174,35 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         ks = __ldg(c.ks + blk);
         vs = __ldg(c.vs + blk);
     }
-    const uint32_t bar0 = smem_addr(bars + warp * AT_STAGES);
-    if (lane < AT_STAGES) mbar_init(bar0 + 8 * lane, 1);
+    const uint32_t bar0 = smem_addr(bars + warp * STAGES);
+    if (lane < STAGES) mbar_init(bar0 + 8 * lane, PB);
     fence_mbar_init();
     __syncwarp();
     // a ring of block copies per warp; lane i issues block i's, the first of
     // them under q's preparation
-    const uint32_t ring = smem_addr(at_sm) + warp * (AT_STAGES * Cfg::STAGE);
-    auto issue = [&](int i) {
-        if (lane == i) {
-            const uint32_t bar = bar0 + 8 * (i % AT_STAGES), dst = ring + (i % AT_STAGES) * Cfg::STAGE;
-            mbar_expect_tx_relaxed(bar, Cfg::STAGE);
-            bulk_g2s(dst, c.k + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
-            bulk_g2s(dst + KV8_BLOCK * HD, c.v + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
+    const uint32_t ring = smem_addr(at_sm) + warp * (STAGES * Cfg::STAGE);
+    const int ni = (nb + PB - 1) / PB;           // iterations
+    auto issue = [&](int i, int st) {
+        if (lane / PB == i) {
+            const uint32_t bar = bar0 + 8 * st, dst = ring + st * Cfg::STAGE + lane % PB * Cfg::BLOCK;
+            if (lane < nb) {
+                mbar_expect_tx_relaxed(bar, Cfg::BLOCK);
+                bulk_g2s(dst, c.k + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
+                bulk_g2s(dst + KV8_BLOCK * HD, c.v + blk * (KV8_BLOCK * HD), KV8_BLOCK * HD, bar);
+            } else {
+                mbar_arrive(bar);
+            }
         }
     };
-    for (int i = 0; i < AT_STAGES && i < nb; ++i) issue(i);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+        if (i < ni) issue(i, i);
+    // V's scales relative to the largest of the warp's blocks, the unit of its
+    // accumulator
+    float vref = vs;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, d));
+    const float vrel = vref > 0.0f ? __fdiv_rn(vs, vref) : 0.0f;
 
     // ---- q: rows rotated at their positions, scaled by a power of two, as fragments
     const T *q = static_cast<const T *>(a.q);
@@ -211,8 +227,9 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         store4(qrow + r * HD + oct_b(o, HD, neox), x.b[0], x.b[1], x.b[2], x.b[3]);
     }
     __syncthreads();
-    // A row becomes 24-bit integers of its largest magnitude / (127 2^16), in
-    // three signed base-256 digits: products with the codes are then exact s8
+    // A row becomes integers of its largest magnitude / Q_TOP, in three signed
+    // base-256 digits (two for f16 callers: 2^-16 of the largest, where their
+    // own q carries 2^-11 of each): products with the codes are then exact s8
     // MMAs on the codes as they are, and a score is as good as from f32 q.
     for (int r = warp; r < R; r += AT_WARPS) {
         float m = 0.0f, zero = 0.0f;
@@ -227,8 +244,8 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         }
         if (lane == 0) {
             m = fmaxf(m, 1e-30f);                             // smaller rows count as zero
-            qinv[r] = __fdiv_rn(Q_TOP, m);
-            rscale[r] = __fdiv_rn(m, Q_TOP) + zero;
+            qinv[r] = __fdiv_rn(Cfg::Q_TOP, m);
+            rscale[r] = __fdiv_rn(m, Cfg::Q_TOP) + zero;
             if (r < rows) {
                 const int t = (rt * R + r) / group, p = s.len - s.n_new + t;
                 row_pos[r] = p;
@@ -255,13 +272,14 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
             const float4 f = *reinterpret_cast<const float4 *>(qrow + r * HD + d);
             const int q0 = __float2int_rn(f.x * inv), q1 = __float2int_rn(f.y * inv), q2 = __float2int_rn(f.z * inv),
                       q3 = __float2int_rn(f.w * inv);
-            // digits of x: its bytes, each carrying into the next where the
-            // lower one counts as negative
-            const int a0 = q0 + 0x8080, a1 = q1 + 0x8080, a2 = q2 + 0x8080, a3 = q3 + 0x8080;
+            // digits: the bytes, each carrying into the next where the lower
+            // one counts as negative; the highest first
+            constexpr int carry = DIGITS == 3 ? 0x8080 : 0x80;
+            const int a0 = q0 + carry, a1 = q1 + carry, a2 = q2 + carry, a3 = q3 + carry;
             const uint32_t l01 = prmt(a0, a1, 0x5140), l23 = prmt(a2, a3, 0x5140);       // bytes 0, 0, 1, 1
             const uint32_t h01 = prmt(a0, a1, 0x0062), h23 = prmt(a2, a3, 0x0062);       // bytes 2, 2
-            word[k] = make_uint4(prmt(h01, h23, 0x5410), prmt(l01, l23, 0x7632) ^ 0x80808080u,
-                                 prmt(l01, l23, 0x5410) ^ 0x80808080u, 0);
+            const uint32_t b0 = prmt(l01, l23, 0x5410) ^ 0x80808080u, b1 = prmt(l01, l23, 0x7632), b2 = prmt(h01, h23, 0x5410);
+            word[k] = DIGITS == 3 ? make_uint4(b2, b1 ^ 0x80808080u, b0, 0) : make_uint4(b1, b0, 0, 0);
         }
         __syncthreads();
 #pragma unroll
@@ -302,7 +320,6 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
-    float vref = 0.0f;                   // the V scale the accumulator is in units of
     // the keys every row of the tile sees need no mask
     int all_lo = 0, all_hi = INT_MAX;
     for (int r = 0; r < rows; ++r) {
@@ -310,48 +327,56 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         all_hi = min(all_hi, row_hi[r]);
     }
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const int key_end = (b0 + nb) * KV8_BLOCK;
+    all_hi = min(all_hi, key_end);
     bool ok = true;
     int i = 0, st = 0;
     uint32_t phase = 0;
-    for (; i < nb; ++i) {
+    for (; i < ni; ++i) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * st, phase))) {
             ok = false;
             break;
         }
-        const uint32_t kbuf = ring + st * Cfg::STAGE, vbuf = kbuf + KV8_BLOCK * HD;
-        const int b = b0 + i;
-        const float kscale = __shfl_sync(0xffffffffu, ks, i), vscale = __shfl_sync(0xffffffffu, vs, i);
+        const uint32_t buf = ring + st * Cfg::STAGE;
+        const int k0 = (b0 + i * PB) * KV8_BLOCK;    // first key
+        float z[PB][NT][4], kscale[PB], vr[PB];
+#pragma unroll
+        for (int h = 0; h < PB; ++h) {
+            kscale[h] = __shfl_sync(0xffffffffu, ks, i * PB + h);
+            vr[h] = __shfl_sync(0xffffffffu, vrel, i * PB + h);
+        }
         // S^T: 16 keys x R rows, each digit of q in an accumulator of its own
         // that starts at the bits of 1.5 2^23: the sums (below 2^22) then are
         // the floats 1.5 2^23 + sum
-        float z[NT][4];
-        {
-            int acc[3][NT][4];
 #pragma unroll
-            for (int d = 0; d < 3; ++d)
+        for (int h = 0; h < PB; ++h) {
+            const uint32_t kbuf = buf + h * Cfg::BLOCK;
+            int acc[DIGITS][NT][4];
+#pragma unroll
+            for (int d = 0; d < DIGITS; ++d)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[d][nt][e] = 0x4b400000;
 #pragma unroll
             for (int ch = 0; ch < KW / WPC; ++ch) {
-                uint32_t k0[WPC], k1[WPC];
-                lds_words<WPC>(kbuf + gq * HD + ch * (16 * WPC) + tq * (4 * WPC), k0);
-                lds_words<WPC>(kbuf + (gq + 8) * HD + ch * (16 * WPC) + tq * (4 * WPC), k1);
+                uint32_t x0[WPC], x1[WPC];
+                lds_words<WPC>(kbuf + gq * HD + ch * (16 * WPC) + tq * (4 * WPC), x0);
+                lds_words<WPC>(kbuf + (gq + 8) * HD + ch * (16 * WPC) + tq * (4 * WPC), x1);
 #pragma unroll
                 for (int e = 0; e < WPC; e += 2) {
                     const int w = ch * WPC + e;
-                    const uint32_t af[4] = {k0[e], k1[e], k0[e + 1], k1[e + 1]};
+                    const uint32_t af[4] = {x0[e], x1[e], x0[e + 1], x1[e + 1]};
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         if constexpr (Cfg::Q_REGS) {
 #pragma unroll
-                            for (int d = 0; d < 3; ++d) mma_s8(acc[d][nt], af, qreg[w][d], qreg[w + 1][d]);
+                            for (int d = 0; d < DIGITS; ++d) mma_s8(acc[d][nt], af, qreg[w][d], qreg[w + 1][d]);
                         } else {
-                            const uint4 f = qf[(w * NT + nt) * 32 + lane], h = qf[((w + 1) * NT + nt) * 32 + lane];
-                            mma_s8(acc[0][nt], af, f.x, h.x);
-                            mma_s8(acc[1][nt], af, f.y, h.y);
-                            mma_s8(acc[2][nt], af, f.z, h.z);
+                            const uint4 f = qf[(w * NT + nt) * 32 + lane], g4 = qf[((w + 1) * NT + nt) * 32 + lane];
+                            mma_s8(acc[0][nt], af, f.x, g4.x);
+                            mma_s8(acc[1][nt], af, f.y, g4.y);
+                            if constexpr (DIGITS == 3) mma_s8(acc[2][nt], af, f.z, g4.z);
                         }
                     }
                 }
@@ -360,63 +385,62 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float f0 = __int_as_float(acc[0][nt][e]) - 12582912.0f, f1 = __int_as_float(acc[1][nt][e]) - 12582912.0f,
-                                f2 = __int_as_float(acc[2][nt][e]) - 12582912.0f;
-                    z[nt][e] = fmaf(f0, 65536.0f, fmaf(f1, 256.0f, f2));
+                    float f = __int_as_float(acc[0][nt][e]) - 12582912.0f;
+#pragma unroll
+                    for (int d = 1; d < DIGITS; ++d) f = fmaf(f, 256.0f, __int_as_float(acc[d][nt][e]) - 12582912.0f);
+                    z[h][nt][e] = f;
                 }
         }
-        // V's codes on their way to registers under the scores and weights
-        uint32_t vw[Cfg::V_EARLY ? 4 : 1][Cfg::V_EARLY ? VW : 1];
-        const uint32_t vp = vbuf + 2 * tq * HD + gq * (HD / 8);
-        if constexpr (Cfg::V_EARLY) {
-#pragma unroll
-            for (int ch = 0; ch < VW / VL; ++ch)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    lds_words<VL>(vp + ((r & 1) + 8 * (r >> 1)) * HD + ch * (4 * VL), *reinterpret_cast<uint32_t (*)[VL]>(&vw[r][ch * VL]));
-        }
-        const int j0 = b * KV8_BLOCK + gq;           // this thread's keys: j0 and j0 + 8
-        const bool masked = (b << 4) < all_lo || (b << 4) + 16 > all_hi;
-        bool grow = vscale > vref;
+        const bool masked = k0 < all_lo || k0 + PB * KV8_BLOCK > all_hi;
         // y = z - m in powers of two; hidden keys -inf
         if (mods) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int h = 0; h < PB; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
-                    float x = z[nt][e] * (rs[nt][e & 1] * kscale);
-                    if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
-                    z[nt][e] = fmaf(x, LOG2E, -fmaf(row_slope[r], fabsf((float)(row_pos[r] - j)), mrun[nt][e & 1]));
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = nt * 8 + 2 * tq + (e & 1), j = k0 + h * KV8_BLOCK + gq + 8 * (e >> 1);
+                        float x = z[h][nt][e] * (rs[nt][e & 1] * kscale[h]);
+                        if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
+                        z[h][nt][e] = fmaf(x, LOG2E, -fmaf(row_slope[r], fabsf((float)(row_pos[r] - j)), mrun[nt][e & 1]));
+                    }
         } else {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int h = 0; h < PB; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[nt][e] = fmaf(z[nt][e], rs[nt][e & 1] * kscale, -mrun[nt][e & 1]);
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        z[h][nt][e] = fmaf(z[h][nt][e], rs[nt][e & 1] * kscale[h], -mrun[nt][e & 1]);
         }
         if (masked) {
 #pragma unroll
+            for (int h = 0; h < PB; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = nt * 8 + 2 * tq + (e & 1), j = k0 + h * KV8_BLOCK + gq + 8 * (e >> 1);
+                        if (j < row_lo[r] || j >= row_hi[r] || j >= key_end) z[h][nt][e] = -INFINITY;
+                    }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int h = 0; h < PB; ++h)
+#pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = nt * 8 + 2 * tq + (e & 1), j = j0 + 8 * (e >> 1);
-                    if (j < row_lo[r] || j >= row_hi[r]) z[nt][e] = -INFINITY;
-                }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) grow |= z[nt][e] > thr[nt][e & 1];
+                for (int e = 0; e < 4; ++e) grow |= z[h][nt][e] > thr[nt][e & 1];
         if (__any_sync(0xffffffffu, grow)) {
-            // new maxima (over the 16 keys: lanes with the same tq) and V unit
-            const float vnew = fmaxf(vref, vscale), vf = vnew > 0.0f ? __fdividef(vref, vnew) : 0.0f;
-            vref = vnew;
+            // new maxima over the keys: lanes with the same tq
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float up = fmaxf(z[nt][e], z[nt][e + 2]), f = vf;
+                    float up = fmaxf(z[0][nt][e], z[0][nt][e + 2]), f = 1.0f;
+#pragma unroll
+                    for (int h = 1; h < PB; ++h) up = fmaxf(up, fmaxf(z[h][nt][e], z[h][nt][e + 2]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, d));
                     if (thr[nt][e] == LOWEST) {
@@ -424,13 +448,15 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
                         else up = 0.0f;
                     } else {
                         up = fmaxf(up, 0.0f);
-                        const float g1 = ex2(-up);
-                        lsum[nt][e] *= g1;
-                        f *= g1;
+                        f = ex2(-up);
+                        lsum[nt][e] *= f;
                     }
                     mrun[nt][e] += up;
-                    z[nt][e] -= up;
-                    z[nt][e + 2] -= up;
+#pragma unroll
+                    for (int h = 0; h < PB; ++h) {
+                        z[h][nt][e] -= up;
+                        z[h][nt][e + 2] -= up;
+                    }
 #pragma unroll
                     for (int mt = 0; mt < HD / 16; ++mt) {
                         o[mt][nt][e] *= f;
@@ -438,60 +464,58 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
                     }
                 }
         }
-        // weights, in units of the running V scale for the second product
-        const float vr = vref > 0.0f ? __fdividef(vscale, vref) : 0.0f;
-        uint32_t pf[NT][PARTS][2];
+        // weights, in units of the warp's V scale for the second product
+        uint32_t pf[PB][NT][PARTS][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float w[4];
+        for (int h = 0; h < PB; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = ex2(z[nt][e]);
-                lsum[nt][e & 1] += p;
-                w[e] = p * vr;
-            }
-            const uint32_t h0 = half2_bits(w[0], w[1]), h1 = half2_bits(w[2], w[3]);
-            pf[nt][0][0] = movm_t(h0);
-            pf[nt][0][1] = movm_t(h1);
-            if constexpr (SPLIT) {
-                pf[nt][1][0] = movm_t(half2_bits(w[0] - h2f(h0 & 0xffffu), w[1] - h2f(h0 >> 16)));
-                pf[nt][1][1] = movm_t(half2_bits(w[2] - h2f(h1 & 0xffffu), w[3] - h2f(h1 >> 16)));
-            }
-        }
-        // O^T += V^T P^T: a word holds four channels, two per m tile
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
 #pragma unroll
-        for (int ch = 0; ch < VW / VL; ++ch) {
-            uint32_t v[4][VL];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if constexpr (Cfg::V_EARLY) {
-#pragma unroll
-                    for (int e = 0; e < VL; ++e) v[r][e] = vw[r][ch * VL + e];
-                } else {
-                    lds_words<VL>(vp + ((r & 1) + 8 * (r >> 1)) * HD + ch * (4 * VL), v[r]);
+                for (int e = 0; e < 4; ++e) {
+                    const float p = ex2(z[h][nt][e]);
+                    lsum[nt][e & 1] += p;
+                    w[e] = p * vr[h];
+                }
+                const uint32_t h0 = half2_bits(w[0], w[1]), h1 = half2_bits(w[2], w[3]);
+                pf[h][nt][0][0] = movm_t(h0);
+                pf[h][nt][0][1] = movm_t(h1);
+                if constexpr (SPLIT) {
+                    pf[h][nt][1][0] = movm_t(half2_bits(w[0] - h2f(h0 & 0xffffu), w[1] - h2f(h0 >> 16)));
+                    pf[h][nt][1][1] = movm_t(half2_bits(w[2] - h2f(h1 & 0xffffu), w[3] - h2f(h1 >> 16)));
                 }
             }
+        // O^T += V^T P^T: a word holds four channels, two per m tile
 #pragma unroll
-            for (int e = 0; e < VL; ++e) {
-                const int w = ch * VL + e;
-                const uint32_t p0 = v[0][e] ^ 0x80808080u, p1 = v[1][e] ^ 0x80808080u, p2 = v[2][e] ^ 0x80808080u,
-                               p3 = v[3][e] ^ 0x80808080u;
-                const uint32_t x0 = prmt(p0, p1, 0x5140), x1 = prmt(p0, p1, 0x7362);
-                const uint32_t y0 = prmt(p2, p3, 0x5140), y1 = prmt(p2, p3, 0x7362);
-                const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
-                const uint32_t hi[4] = {code_pair(x1, 0x4140), code_pair(x1, 0x4342), code_pair(y1, 0x4140), code_pair(y1, 0x4342)};
+        for (int h = 0; h < PB; ++h) {
+            const uint32_t vp = buf + h * Cfg::BLOCK + KV8_BLOCK * HD + 2 * tq * HD + gq * (HD / 8);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int ch = 0; ch < VW / VL; ++ch) {
+                uint32_t v[4][VL];
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        mma_f16(o[2 * w][nt], lo, pf[nt][p][0], pf[nt][p][1]);
-                        mma_f16(o[2 * w + 1][nt], hi, pf[nt][p][0], pf[nt][p][1]);
-                    }
+                for (int r = 0; r < 4; ++r) lds_words<VL>(vp + ((r & 1) + 8 * (r >> 1)) * HD + ch * (4 * VL), v[r]);
+#pragma unroll
+                for (int e = 0; e < VL; ++e) {
+                    const int w = ch * VL + e;
+                    const uint32_t p0 = v[0][e] ^ 0x80808080u, p1 = v[1][e] ^ 0x80808080u, p2 = v[2][e] ^ 0x80808080u,
+                                   p3 = v[3][e] ^ 0x80808080u;
+                    const uint32_t x0 = prmt(p0, p1, 0x5140), x1 = prmt(p0, p1, 0x7362);
+                    const uint32_t y0 = prmt(p2, p3, 0x5140), y1 = prmt(p2, p3, 0x7362);
+                    const uint32_t lo[4] = {code_pair(x0, 0x4140), code_pair(x0, 0x4342), code_pair(y0, 0x4140), code_pair(y0, 0x4342)};
+                    const uint32_t hi[4] = {code_pair(x1, 0x4140), code_pair(x1, 0x4342), code_pair(y1, 0x4140), code_pair(y1, 0x4342)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            mma_f16(o[2 * w][nt], lo, pf[h][nt][p][0], pf[h][nt][p][1]);
+                            mma_f16(o[2 * w + 1][nt], hi, pf[h][nt][p][0], pf[h][nt][p][1]);
+                        }
+                }
             }
         }
         __syncwarp();                        // every lane has read the stage
-        if (i + AT_STAGES < nb) issue(i + AT_STAGES);
-        if (++st == AT_STAGES) {
+        if (i + STAGES < ni) issue(i + STAGES, st);
+        if (++st == STAGES) {
             st = 0;
             phase ^= 1;
         }
@@ -499,8 +523,8 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     if (!ok) {
         // a copy did not arrive in time: report it, and leave no copy in flight
         if (lane == 0) atomicOr(a.status, STATUS_WAIT_TIMEOUT);
-        for (int k = i; k < min(i + AT_STAGES, nb); ++k)
-            (void)mbar_wait(bar0 + 8 * (k % AT_STAGES), (k / AT_STAGES) & 1, 200000000ull);
+        for (int k = i; k < min(i + STAGES, ni); ++k)
+            (void)mbar_wait(bar0 + 8 * (k % STAGES), (k / STAGES) & 1, 200000000ull);
     }
 
     // ---- the four warps' parts, then this CTA's
@@ -639,12 +663,14 @@ AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     g.row_tiles = (int)((rows + R - 1) / R);
     g.rows = (int)(rows < R ? rows : R);
     // Keys per CTA: a CTA's preparation of q and its join cost as much as some
-    // tens of blocks, so as many keys as leave three CTAs per SM, at most a
-    // warp's 32 blocks each (2048 keys against 1024 and 512, one 131K-token
-    // request at the Qwen2.5-32B shape: 81, 99 and 125 us; 64 requests of 4250
-    // tokens at the Llama-3-8B shape: 126, 128 and 150 us), at least 256.
-    const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, want = 3 * (int64_t)num_sms;
-    int64_t splits = (want + units - 1) / units;
+    // tens of blocks, so as many keys as a warp's 32 blocks allow (2048 per
+    // CTA; 1024 and 512 took 99 and 125 us where 2048 took 81: one 131K-token
+    // request at the Qwen2.5-32B shape), at least 256, in whole rounds of the
+    // GPU's three CTAs per SM.
+    const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, slots = 3 * (int64_t)num_sms;
+    const int64_t least = (a.max_len + AT_CHUNK - 1) / AT_CHUNK, rounds = (units * least + slots - 1) / slots;
+    int64_t splits = rounds * slots / units;
+    if (splits < least) splits = least;
     int64_t chunk = (a.max_len + splits - 1) / splits;
     if (chunk < 256) chunk = 256;
     chunk = (chunk + 63) / 64 * 64;
