@@ -593,7 +593,7 @@ typedef struct sicu_kv8_attn {
     const int32_t *first;         /* [n_seq] or NULL */
     const sicu_rope_tables *rope; /* host struct, or NULL */
 } sicu_kv8_attn;
-/* Workspace bytes for a call with these sizes (pointers are not looked at);
+/* Workspace bytes for a call with these sizes (of pointers only whether prefix is given counts);
  * ws is 16-byte aligned and belongs to the call until it has run. */
 SICU_API int sicu_kv8_attention_ws(const sicu_kv8 *cache, const sicu_kv8_attn *a, size_t *bytes);
 SICU_API int sicu_kv8_attention(const sicu_kv8 *cache, const sicu_kv8_attn *a, const void *dq, void *dout, void *ws,

@@ -1431,6 +1431,7 @@ static int check_kv8_attn(const Kv8Dev &c, const sicu_kv8_attn *a, Kv8AttnDev &d
     d.scale = a->scale;
     d.cap = a->cap;
     d.window = a->window > a->max_len ? 0 : (int)a->window;
+    d.prefix = a->prefix;                // whether there is one: the workspace's size depends on it
     return SICU_OK;
 }
 

@@ -62,7 +62,9 @@ __device__ __forceinline__ float ex2(float x) {
 // few 2^-23 of the cap, saturating without overflow
 __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
     const float e = ex2(x * inv_cap * (2.0f * LOG2E));
-    return cap - 2.0f * cap * __fdividef(1.0f, 1.0f + fminf(e, 1e30f));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return fmaf(-2.0f * cap, r, cap);
 }
 
 // weight of a part with maximum mp under the joint maximum m: parts that saw
@@ -148,8 +150,8 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     float *qrow = reinterpret_cast<float *>(at_sm + Cfg::MAIN);
     uint4 *qf = reinterpret_cast<uint4 *>(qrow);
     __shared__ float rscale[R], qinv[R], sm_m[AT_WARPS][R], sm_l[AT_WARPS][R], sm_vr[AT_WARPS];
-    __shared__ int row_lo[R], row_hi[R], row_pos[R];
-    __shared__ float row_slope[R];
+    __shared__ int row_lo[R], row_hi[R];
+    __shared__ float row_slope[R], row_pos[R];   // positions as f32: exact below 2^24, within 2^-24 past it
     __shared__ __align__(8) uint64_t bars[AT_WARPS * STAGES];
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the combine, which waits for this grid
@@ -248,13 +250,13 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
             rscale[r] = __fdiv_rn(m, Cfg::Q_TOP) + zero;
             if (r < rows) {
                 const int t = (rt * R + r) / group, p = s.len - s.n_new + t;
-                row_pos[r] = p;
+                row_pos[r] = (float)p;
                 row_lo[r] = kv8_lo(a, s, p);
                 row_hi[r] = kv8_hi(s, p);
                 row_slope[r] = a.slopes ? __ldg(a.slopes + head * group + (rt * R + r) % group) * LOG2E : 0.0f;
             } else {
-                row_pos[r] = row_lo[r] = row_hi[r] = 0;
-                row_slope[r] = 0.0f;
+                row_lo[r] = row_hi[r] = 0;
+                row_pos[r] = row_slope[r] = 0.0f;
             }
         }
     }
@@ -394,17 +396,25 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
         const bool masked = k0 < all_lo || k0 + PB * KV8_BLOCK > all_hi;
         // y = z - m in powers of two; hidden keys -inf
         if (mods) {
+            const float j0 = (float)(k0 + gq);
 #pragma unroll
-            for (int h = 0; h < PB; ++h)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 2; ++e) {
+                    const int r = nt * 8 + 2 * tq + e;
+                    const float slope = row_slope[r], dist = row_pos[r] - j0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = nt * 8 + 2 * tq + (e & 1), j = k0 + h * KV8_BLOCK + gq + 8 * (e >> 1);
-                        float x = z[h][nt][e] * (rs[nt][e & 1] * kscale[h]);
-                        if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
-                        z[h][nt][e] = fmaf(x, LOG2E, -fmaf(row_slope[r], fabsf((float)(row_pos[r] - j)), mrun[nt][e & 1]));
+                    for (int h = 0; h < PB; ++h) {
+                        const float cs = rs[nt][e] * kscale[h];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            float x = z[h][nt][e + 2 * u] * cs;
+                            if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
+                            x = fmaf(x, LOG2E, -mrun[nt][e]);
+                            z[h][nt][e + 2 * u] = fmaf(-slope, fabsf(dist - (float)(h * KV8_BLOCK + 8 * u)), x);
+                        }
                     }
+                }
         } else {
 #pragma unroll
             for (int h = 0; h < PB; ++h)
@@ -590,13 +600,15 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
     }
 }
 
-// Joins the splits of a row: one CTA per row, its warps take every fourth split
-// and are added in order.
+// Joins the splits of a row: one CTA per row, its warps deal the splits among
+// them and are added in order. A row's 108 splits (one request of 131K tokens)
+// took four warps 27 us, a load's latency at a time.
+constexpr int COMB_WARPS = 16;
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, int R, const float *ws) {
+__global__ void __launch_bounds__(COMB_WARPS * 32) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, int R, const float *ws) {
     constexpr int E = HD / 32;
-    __shared__ float acc_sm[4][HD], l_sm[4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ float acc_sm[COMB_WARPS][HD], l_sm[COMB_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int head = blockIdx.x % c.hkv, rt = blockIdx.x / c.hkv, r = blockIdx.y, seq = blockIdx.z;
     const Kv8Seq s = kv8_seq(a, seq);
     const int group = a.n_head / c.hkv, n_rows = s.n_new * group;
@@ -607,31 +619,49 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8Dev c, Kv8AttnDev a
     if (parts <= 1 || r >= rows) return;
     const int64_t stride = part_floats(g.rows, HD);
     const float *p0 = ws + part_index(g, c.hkv, seq, head, rt, 0) * stride;
+    const float *o0 = p0 + r * HD + lane, *ml0 = p0 + g.rows * HD + 2 * r;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p0[i * stride + g.rows * HD + 2 * r]);
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml0[i * stride]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     float l = 0.0f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (int i = warp; i < parts; i += 4) {
-        const float *p = p0 + i * stride;
-        const float f = join(p[g.rows * HD + 2 * r], m);
-        l += p[g.rows * HD + 2 * r + 1] * f;
+    constexpr int U = 4;                 // splits whose loads are in flight
+    for (int i = warp; i < parts; i += U * warps) {
+        float f[U], li[U], x[U][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += p[r * HD + e * 32 + lane] * f;
+        for (int u = 0; u < U; ++u) {
+            const int k = min(i + u * warps, parts - 1);
+            f[u] = ml0[k * stride];
+            li[u] = ml0[k * stride + 1];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = o0[k * stride + e * 32];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u * warps >= parts) break;
+            const float w = join(f[u], m);
+            l += li[u] * w;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += x[u][e] * w;
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) acc_sm[warp][e * 32 + lane] = acc[e];
     if (lane == 0) l_sm[warp] = l;
     __syncthreads();
-    const float inv = inv_sum(l_sm[0] + l_sm[1] + l_sm[2] + l_sm[3]);
+    float sum = 0.0f;
+    for (int w = 0; w < warps; ++w) sum += l_sm[w];
+    const float inv = inv_sum(sum);
     const int rr = rt * R + r, t = rr / group, h = head * group + rr % group;
     T *out = static_cast<T *>(a.out) + (int64_t)(s.t0 + t) * a.out_stride + (int64_t)h * HD;
-    for (int d = threadIdx.x; d < HD; d += 128)
-        store1(out + d, (acc_sm[0][d] + acc_sm[1][d] + acc_sm[2][d] + acc_sm[3][d]) * inv);
+    for (int d = threadIdx.x; d < HD; d += blockDim.x) {
+        float x = 0.0f;
+        for (int w = 0; w < warps; ++w) x += acc_sm[w][d];
+        store1(out + d, x * inv);
+    }
 }
 
 // The rows (query heads of one KV head x new tokens) up to which a request
@@ -668,16 +698,19 @@ AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     // request at the Qwen2.5-32B shape), at least 256, in whole rounds of the
     // GPU's three CTAs per SM.
     const int64_t units = (int64_t)a.n_seq * c.hkv * g.row_tiles, slots = 3 * (int64_t)num_sms;
-    const int64_t least = (a.max_len + AT_CHUNK - 1) / AT_CHUNK, rounds = (units * least + slots - 1) / slots;
+    // the keys a row tile can see: a window bounds them, unless a prefix does not
+    int64_t most = a.max_len;
+    if (a.window > 0 && !a.prefix && (int64_t)a.window + a.max_new < most) most = (int64_t)a.window + a.max_new;
+    const int64_t least = (most + AT_CHUNK - 1) / AT_CHUNK, rounds = (units * least + slots - 1) / slots;
     int64_t splits = rounds * slots / units;
     if (splits < least) splits = least;
-    int64_t chunk = (a.max_len + splits - 1) / splits;
+    int64_t chunk = (most + splits - 1) / splits;
     if (chunk < 256) chunk = 256;
     chunk = (chunk + 63) / 64 * 64;
     if (chunk > AT_CHUNK) chunk = AT_CHUNK;
     g.chunk = (int)chunk;
     // a span rounded down to a block may begin 15 keys early
-    g.splits = (int)((a.max_len + 15 + chunk - 1) / chunk);
+    g.splits = (int)((most + 15 + chunk - 1) / chunk);
     return g;
 }
 
@@ -691,7 +724,8 @@ int launch_typed(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float 
     if (g.splits > 1) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(g.row_tiles * c.hkv), (unsigned)g.rows, (unsigned)a.n_seq);
-        cfg.blockDim = dim3(128);
+        // a warp for every few splits
+        cfg.blockDim = dim3(g.splits <= 4 ? 64 : g.splits <= 16 ? 128 : COMB_WARPS * 32);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
