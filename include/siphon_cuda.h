@@ -545,7 +545,7 @@ SICU_API int sicu_kv8_release(const int32_t *drop, int32_t *len, int64_t n_seq, 
  * rope is given (NULL: not). Tokens of one 16-token block are adjacent and in
  * ascending order, as sicu_kv8_plan lists them, and rows of a block before the
  * first of them are valid. A negative slot's token is skipped. A block's scale
- * becomes s = max(s, max|x| / 127) over the rows given (from 0 when they begin
+ * becomes s = max(s, max|x| * (1 / 127 in f32)) over the rows given (from 0 when they begin
  * the block), rows stored earlier are requantized when it grows (rint(code *
  * (s_old * (1 / s)))), and each row becomes rint(x * (1 / s)). Magnitudes
  * below 2^-112 count as 0. A value that is not finite does not enter the scale:

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_release_kernel(const int32_t
 
 // ---- store ---------------------------------------------------------------------------
 //
-// A block's scale is the largest |x| it was given over 127; code = rne(x /
+// A block's scale is the largest |x| it was given times fl(1 / 127); code = rne(x /
 // scale). Rows appended to a block that already holds some may need a larger
 // scale: the codes in place are then requantized to it (rne(code * old / new)),
 // each at most once per doubling of the scale in practice. Two warps own one
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(STORE_WARPS * 32, HD <= 128 ? 5 : 3) kv8_store
         asm volatile("bar.sync %0, 64;" :: "r"(1 + pair) : "memory");
         amax = fmaxf(amax, top[parity][warp ^ 1]);
         if (!in) continue;
-        const float sc = fmaxf(before, amax >= KV8_TINY ? __fdiv_rn(amax, 127.0f) : 0.0f);
+        const float sc = fmaxf(before, amax >= KV8_TINY ? __fmul_rn(amax, 1.0f / 127.0f) : 0.0f);
         const float inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
         if (sc > before && lead > 0) {
             // rows stored earlier: their codes at the larger scale

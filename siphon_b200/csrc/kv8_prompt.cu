@@ -37,6 +37,15 @@ constexpr int PT_THREADS = 512;       // softmax 2 x 4 warps, converters 7, MMA 
 constexpr int PT_W_CONV = 8, PT_W_MMA = 15, PT_NCONV = 7;
 constexpr int PT_BUF = 3;             // f16 tiles: K and V of successive key tiles take turns
 constexpr int PT_RING = 4;            // tiles whose scales are kept
+// The tensor cores drop bits of an f32 sum at every step of 16 keys, always
+// toward zero: some 1.2e-8 of it, and twice the steps with weights in two
+// parts. For f32 callers the output's sums start anew every 16 tiles, the
+// finished ones added up in the output rows: relative error 2.9e-6 for an
+// 8191-token prompt at the Llama-3-8B shape, where it was 6.2e-6 and growing with
+// the context (an f32 computation's is 1.1e-6), for 12 % of that prompt's time
+// (861 -> 964 us). f16 callers' results stay below their own rounding up to
+// 128 K keys without.
+constexpr int PT_FLUSH = 16;
 
 // Barriers. The converters fill the three tile buffers in the order K0 V0 K1
 // V1 ...: V of tile j then waits only for the scores of tile j (K's release),
@@ -435,6 +444,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             const float rs = rsv[r], cap_in = a.cap > 0.0f ? 1.0f / a.cap : 0.0f, cap2 = a.cap * LOG2E;
             const float slope = a.slopes ? __ldg(a.slopes + h) * LOG2E : 0.0f;
             float m = 0.0f, thr = LOWEST, l = 0.0f;
+            float kept = 1.0f;           // the output rows' factor since they were written
+            const int tok = (r0 + r) / group;
+            const int64_t row_at = (int64_t)(s.t0 + tok) * a.out_stride + (int64_t)(head * group + r0 + r - tok * group) * HD;
             bool ok = true;
             for (int j = 0; j < nj; ++j) {
                 if (!__all_sync(ALL, pt_wait(bar(B_SC + j % PT_RING), (uint32_t)(j / PT_RING) & 1u, abort_flag, a.status) &&
@@ -443,6 +455,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                     break;
                 }
                 tc_fence_after();
+                if constexpr (SPLIT) {
+                    // S of this tile is complete, so every product before it is
+                    if (j > 0 && j % PT_FLUSH == 0) {
+                        float *dst = reinterpret_cast<float *>(out) + row_at;
+#pragma unroll 1
+                        for (int q = 0; q < HD; q += 16) {
+                            uint32_t w[16];
+                            tmem_ld16(to + q, w);
+                            tmem_wait_ld(w);
+                            if (live) {
+#pragma unroll
+                                for (int e = 0; e < 16; e += 4) {
+                                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                    if (j > PT_FLUSH) x = *reinterpret_cast<const float4 *>(dst + q + e);
+                                    x.x = fmaf(x.x, kept, __uint_as_float(w[e]));
+                                    x.y = fmaf(x.y, kept, __uint_as_float(w[e + 1]));
+                                    x.z = fmaf(x.z, kept, __uint_as_float(w[e + 2]));
+                                    x.w = fmaf(x.w, kept, __uint_as_float(w[e + 3]));
+                                    *reinterpret_cast<float4 *>(dst + q + e) = x;
+                                }
+                            }
+                        }
+                        kept = 1.0f;
+                    }
+                }
                 uint32_t v[4][32];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, v[q]);
@@ -555,7 +592,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                         thr = mx + LAZY;
                         l *= f;
                     }
-                    if (j > 0) {
+                    kept *= f;
+                    if (SPLIT ? j % PT_FLUSH > 0 : j > 0) {
                         // S of this tile is complete, so every product before it is
 #pragma unroll 1
                         for (int q = 0; q < HD; q += 16) {
@@ -623,6 +661,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                     tmem_ld32(to + q, w);
                     tmem_wait_all();
                     tie32(w);
+                    if constexpr (SPLIT) {
+                        if (nj > PT_FLUSH && live) {
+                            const float *src = reinterpret_cast<const float *>(out) + row_at + q;
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 x = *reinterpret_cast<const float4 *>(src + e);
+                                w[e] = __float_as_uint(fmaf(x.x, kept, __uint_as_float(w[e])));
+                                w[e + 1] = __float_as_uint(fmaf(x.y, kept, __uint_as_float(w[e + 1])));
+                                w[e + 2] = __float_as_uint(fmaf(x.z, kept, __uint_as_float(w[e + 2])));
+                                w[e + 3] = __float_as_uint(fmaf(x.w, kept, __uint_as_float(w[e + 3])));
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += PER) {
                         uint32_t x[4];
@@ -635,8 +686,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                     }
                 }
                 __syncwarp();
-                const int tok = (r0 + r) / group;
-                const int64_t row_at = (int64_t)(s.t0 + tok) * a.out_stride + (int64_t)(head * group + r0 + r - tok * group) * HD;
 #pragma unroll 4
                 for (int i = lane; i < 32 * UNITS; i += 32) {
                     const int rw = i / UNITS, u = i % UNITS;
@@ -720,17 +769,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
         auto scores = [&](int t, int j) {
             const uint64_t q = smem_desc(sb + Lay::OFF_Q + t * 2 * Lay::TILE, 1024, SMEM_SWZ_128B);
             const uint64_t k = smem_desc(x_at(2 * j), 1024, SMEM_SWZ_128B);
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t off = ((kk / 4) * Lay::PANEL + (kk % 4) * 32) >> 4;
-                mma_ss(one, TM_S[t], q + off, k + off, id_s, kk != 0);
-            }
+            // the low parts first: added to the finished sums, each step would
+            // round those once more
             if (q_lo) {
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t off = ((kk / 4) * Lay::PANEL + (kk % 4) * 32) >> 4;
-                    mma_ss(one, TM_S[t], q + (Lay::TILE >> 4) + off, k + off, id_s, 1);
+                    mma_ss(one, TM_S[t], q + (Lay::TILE >> 4) + off, k + off, id_s, kk != 0);
                 }
+            }
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t off = ((kk / 4) * Lay::PANEL + (kk % 4) * 32) >> 4;
+                mma_ss(one, TM_S[t], q + off, k + off, id_s, kk ? 1u : (uint32_t)q_lo);
             }
             commit(one, bar(B_S0 + t));
             if (t == n_mt - 1) commit(one, bar(B_FREE + x_buf(2 * j)));
@@ -752,7 +803,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
 #pragma unroll
                     for (int kk = 0; kk < PT_KEYS / 16; ++kk)
                         mma_ts(one, TM_O[t], TM_S[t] + 64 * part + 8 * kk, v + (uint32_t)(kk * 2048 >> 4), id_o,
-                               part | kk ? 1u : (uint32_t)(j != 0));
+                               part | kk ? 1u : (uint32_t)(SPLIT ? j % PT_FLUSH != 0 : j != 0));
                 if (t == n_mt - 1) commit(one, j + 1 < nj ? bar(B_FREE + x_buf(2 * j + 1)) : bar(B_OUT));
                 if (j + 1 < nj) {
                     if (t == 0) ok = full(2 * j + 2);

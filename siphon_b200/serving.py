@@ -1,0 +1,165 @@
+"""A llama-architecture forward pass for many requests at once, over the paged
+8-bit KV cache.
+
+The reference engine runs one sequence, token by token, over its own f16 cache
+(src/cmd_run.c:275-276, src/engine.c:290-398). ``PagedPath`` packs the new
+tokens of every request of a step (chunks of prompts and single tokens, in any
+mix) into one batch of rows and runs the engine's steps over them: the
+embedding rows, the norms with their residual adds, the products, the output
+norm and the head are the library's m-row entry points (as in
+``MatrixPath.prompt_step``); in place of the one-sequence attention
+
+* ``sicu_kv8_plan`` gives each request the pages it needs and lists every new
+  token's slot and position, on the device;
+* ``sicu_kv8_store`` rotates K and writes K and V to those slots in 8 bits;
+* ``sicu_kv8_attention`` rotates q and attends, each request over its own
+  pages.
+
+Only the last row of each request goes through the output head; the greedy
+choice lands in ``next`` (device memory), from which ``decode`` feeds the next
+step without a host round trip. Results differ from the reference's by the
+cache's 8 bits.
+
+    path = PagedPath(sicu, shape, device, max_seqs=8, max_len=2048, n_pages=512, gguf_path=...)
+    path.step(stream, [len(p) for p in prompts], sum(prompts, []))   # the prompts, all at once
+    while ...: path.decode(stream)                                     # one token per live request
+    path.retire(stream, [3])                                           # request 3 ended: its pages are free
+"""
+
+from __future__ import annotations
+
+from itertools import accumulate
+
+from . import lib as L
+from .model_path import MatrixPath
+from .synth_model import LlamaShape
+
+
+class PagedPath(MatrixPath):
+    """max_seqs requests of up to max_len tokens over a pool of n_pages pages
+    of `page` tokens per layer; up to max_tokens new tokens per step."""
+
+    def __init__(self, sicu, sh: LlamaShape, device, max_seqs: int, max_len: int, n_pages: int, page: int = 32,
+                 max_tokens: int = 512, seed: int = 0, gguf_path=None, packed: bool = False):
+        import torch
+        if max_tokens < 2 or max_seqs < 1:
+            raise ValueError("at least two tokens and one request per step")
+        super().__init__(sicu, sh, device, seed=seed, max_tokens=max_tokens, embed=True, n_ctx=max_len,
+                         gguf_path=gguf_path, packed=packed)
+        self.kc = self.vc = None                       # the one-sequence caches are not used
+        nkv, hd = self.shapes["k"][0] // sh.head_dim, sh.head_dim
+        i32 = dict(dtype=torch.int32, device=device)
+        self.page, self.n_pages, self.max_seqs, self.max_len = page, n_pages, max_seqs, max_len
+        self.max_pages = -(-max_len // page)
+        self.buffers, self.cache = [], []
+        for _ in range(sh.n_layer):
+            b = [torch.zeros(n_pages, nkv, page, hd, dtype=torch.int8, device=device) for _ in range(2)] + \
+                [torch.zeros(n_pages, nkv, page // 16, device=device) for _ in range(2)]
+            self.buffers.append(b)
+            self.cache.append(L.kv8_cache(*b, n_pages, page, nkv, hd))
+        self.table = torch.zeros(max_seqs, self.max_pages, **i32)
+        self.free = torch.arange(n_pages - 1, -1, -1, **i32)      # page 0 on top
+        self.n_free = torch.tensor([n_pages], **i32)
+        self.length = torch.zeros(max_seqs, **i32)
+        self.cu = torch.zeros(max_seqs + 1, **i32)
+        self.slot = torch.zeros(max_tokens, dtype=torch.int64, device=device)
+        self.position = torch.zeros(max_tokens, **i32)
+        self.next = torch.zeros(max_seqs, dtype=torch.int64, device=device)   # each request's greedy choice
+        self.last = torch.empty(max_seqs, sh.n_embd, device=device)
+        self.choice = torch.empty(max_seqs, dtype=torch.int64, device=device)
+        self.rope = L.rope(self.rope_cos, self.rope_sin, max_len, hd, sh.neox)
+        self.ws = torch.empty(16, dtype=torch.uint8, device=device)
+        self.len_host = [0] * max_seqs
+
+    def step(self, stream, fresh, tokens) -> int:
+        """Runs fresh[i] new tokens of each request i (0: none), `tokens` all
+        of them in request order (a list, or an int64 tensor on the device).
+        The logits of each advancing request's last token are rows
+        0, 1, ... of y["head"], its greedy choice next[i]. Returns the number of
+        library calls."""
+        import torch
+        m = sum(fresh)
+        lens = [n + f for n, f in zip(self.len_host, fresh)]
+        live, ends = [i for i, f in enumerate(fresh) if f], list(accumulate(fresh))
+        if len(fresh) != self.max_seqs or min(fresh) < 0 or not 0 < m <= self.tokens.numel() or len(tokens) != m:
+            raise ValueError(f"a step of {m} tokens for {len(fresh)} requests: past the buffers")
+        if max(lens) > self.max_len:
+            raise ValueError(f"a request of {max(lens)} tokens: past {self.max_len}")
+        if sum(-(-n // self.page) for n in lens) > self.n_pages:
+            raise ValueError("not enough free pages")
+        s, h, y, sh = self.s, stream.cuda_stream, self.y, self.sh
+        d, eps, hd = sh.n_embd, sh.rms_eps, sh.head_dim
+        nq, nkv, nff = self.shapes["q"][0], self.shapes["k"][0], self.shapes["gate"][0]
+        xp, xn = self.xp, self.xn
+        with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+            self.tokens[:m].copy_(torch.as_tensor(tokens, dtype=torch.int64))
+            new = torch.tensor(fresh, dtype=torch.int32).to(self.dev)
+            ids = torch.tensor(live, dtype=torch.int64).to(self.dev)
+            rows = torch.tensor([ends[i] - 1 for i in live], dtype=torch.int64).to(self.dev)
+        s.kv8_plan(self.length, new, self.max_seqs, self.page, self.table, self.max_pages, self.free, self.n_pages,
+                   self.n_free, self.n_free, m, self.cu, self.length, self.slot, self.position, stream=h)
+        self.len_host = lens
+        attn = L.kv8_attn(L.T_F32, nq // hd, m, self.table, self.max_pages, self.length, self.cu, self.max_seqs,
+                          max(fresh), max(lens), self.kq_scale, rope=self.rope)
+        need = s.kv8_attention_ws(self.cache[0], attn)
+        if self.ws.numel() < need:
+            with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+                self.ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
+        s.row_to_f32_dev(self.embd_type, self.embd, d, sh.n_vocab, self.tokens, m, xp[0], stream=h)
+        cur, nxt, res, n = 0, 1, None, 3
+        for il in range(len(self.layers)):
+            if res is None:
+                s.rms_norm(xp[cur], self.attn_norm[il], d, m, eps, xn, stream=h)
+            else:
+                s.rms_norm(xp[cur], self.attn_norm[il], d, m, eps, xn, dres=res, dsum=xp[nxt], stream=h)
+                cur, nxt = nxt, cur
+            n += 1 + self._prompt_products(il, ("q", "k", "v"), d, xn, m, h)
+            if self.bias is not None:
+                for name, width in (("q", nq), ("k", nkv), ("v", nkv)):
+                    s.add_bias(y[name], self.bias[il][name], width, m, stream=h)
+                n += 3
+            s.kv8_store(self.cache[il], L.T_F32, y["k"], y["v"], self.slot, m, pos=self.position, rope=self.rope,
+                        stream=h)
+            s.kv8_attention(self.cache[il], attn, y["q"], self.att, self.ws, stream=h)
+            n += 2 + self._prompt_products(il, ("o",), nq, self.att, m, h)
+            s.rms_norm(xp[cur], self.ffn_norm[il], d, m, eps, xn, dres=y["o"], dsum=xp[nxt], stream=h)
+            cur, nxt = nxt, cur
+            n += 1 + self._prompt_products(il, ("gate", "up"), d, xn, m, h)
+            s.swiglu(y["gate"], y["up"], nff, m, self.ffp, stream=h)
+            n += 1 + self._prompt_products(il, ("down",), nff, self.ffp, m, h)
+            res = y["down"]
+        s.rms_norm(xp[cur], self.out_norm, d, m, eps, xn, dres=res, dsum=xp[nxt], stream=h)
+        with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+            torch.index_select(xn, 0, rows, out=self.last[:len(live)])
+        self._prompt_head(self.last, len(live), h)
+        s.argmax(y["head"], self.shapes["head"][0], len(live), self.choice, stream=h)
+        with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+            self.next.index_copy_(0, ids, self.choice[:len(live)])
+        return n + 3
+
+    def decode(self, stream) -> int:
+        """One token for every request that holds some: its last greedy choice."""
+        import torch
+        live = [i for i, n in enumerate(self.len_host) if n]
+        if not live:
+            raise ValueError("no request holds tokens")
+        with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+            tokens = self.next.index_select(0, torch.tensor(live, dtype=torch.int64).to(self.dev))
+        return self.step(stream, [1 if n else 0 for n in self.len_host], tokens)
+
+    def retire(self, stream, requests) -> None:
+        """The requests ended: their pages become free, their places empty."""
+        import torch
+        drop = torch.zeros(self.max_seqs, dtype=torch.int32)
+        for i in requests:
+            drop[i] = 1
+            self.len_host[i] = 0
+        with torch.cuda.stream(stream) if self.dev.type == "cuda" else _nothing():
+            drop = drop.to(self.dev)
+        self.s.kv8_release(drop, self.length, self.max_seqs, self.page, self.table, self.max_pages, self.free,
+                           self.n_pages, self.n_free, stream=stream.cuda_stream)
+
+
+def _nothing():
+    from contextlib import nullcontext
+    return nullcontext()

@@ -66,7 +66,7 @@ class Cache:
                 fin = np.isfinite(rows)
                 amax = np.abs(rows[fin]).max() if fin.any() else np.float32(0)
                 before = self.scale[pg, h, sub] if lead else np.float32(0)
-                s = max(before, np.float32(amax) / np.float32(127) if amax >= 2.0 ** -112 else np.float32(0))
+                s = max(before, np.float32(amax) * (one / np.float32(127)) if amax >= 2.0 ** -112 else np.float32(0))
                 inv = one / s if s > 0 else np.float32(0)
                 blk = self.codes[pg, h, sub * BLOCK:(sub + 1) * BLOCK]
                 if s > before and lead:

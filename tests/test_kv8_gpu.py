@@ -480,3 +480,15 @@ def test_calls_repeat_bit_for_bit_on_another_stream_and_in_a_graph(sicu):
         graph.replay()
         assert (host(out) == first).all()
     assert sicu.status() == 0
+
+
+def test_attention_prompt_f32_precision_over_many_keys(sicu):
+    """A chunk far into a long context: f32 results stay as close to 64 bits as
+    sums in f32 do (the bound of `attend` without its slack for the scores:
+    here every score is small, so the sums over 6000 keys are what can err)."""
+    got, want = attend(sicu, 4, 1, 128, 64, [6000], [40], qmul=0.02, seed=21)
+    # 6000 weights near 1 / 6000 of values of unit size: the result is their
+    # mean, some 1 / sqrt(6000) of them; an f32 sum errs by 2^-24 sqrt(6000) of
+    # its terms' size, the weights by 2^-22 each
+    err = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert err < 2.0 ** -18
