@@ -118,6 +118,28 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnDev &a, int i) {
     if (s.first < 0) s.first = 0;
     return s;
 }
+// tanh x for a score x = z / cap. Up to |x| = 1/2, as capped scores mostly are:
+// x (1 + y g(y)), y = x^2, g a least squares fit on Chebyshev nodes with three
+// terms (f16 callers; absolute error below 2^-22) or four (below 2^-27). Past
+// it 1 - 2 / (1 + e^(2 x)), which near 0 would lose what it subtracts.
+constexpr float TANH3_0 = -0.33326461911201477f, TANH3_1 = 0.13185860216617584f, TANH3_2 = -0.04422925412654877f;
+constexpr float TANH4_0 = -0.33333051204681396f, TANH4_1 = 0.13323938846588135f, TANH4_2 = -0.05292435735464096f,
+                TANH4_3 = 0.01700596883893013f;
+template <bool FINE>
+__device__ __forceinline__ float tanh_poly(float x) {
+    const float y = x * x;
+    float g;
+    if constexpr (FINE) g = fmaf(fmaf(fmaf(y, TANH4_3, TANH4_2), y, TANH4_1), y, TANH4_0);
+    else g = fmaf(fmaf(y, TANH3_2, TANH3_1), y, TANH3_0);
+    return fmaf(x * y, g, x);
+}
+__device__ __forceinline__ float tanh_exp(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.88539008177792681f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return fmaf(-2.0f, r, 1.0f);
+}
+
 // positions row p sees: [lo, hi), empty when lo >= hi
 __device__ __forceinline__ int kv8_lo(const Kv8AttnDev &a, const Kv8Seq &s, int p) {
     const int w = a.window > 0 ? p + 1 - a.window : 0;

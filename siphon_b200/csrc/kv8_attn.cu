@@ -58,15 +58,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// cap * tanh(x / cap) as cap - 2 cap / (1 + e^(2 x / cap)): absolute error a
-// few 2^-23 of the cap, saturating without overflow
-__device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
-    const float e = ex2(x * inv_cap * (2.0f * LOG2E));
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return fmaf(-2.0f * cap, r, cap);
-}
-
 // weight of a part with maximum mp under the joint maximum m: parts that saw
 // no key (both -inf) keep their zero sums, and a NaN sum stays NaN
 __device__ __forceinline__ float join(float mp, float m) { return mp == m ? 1.0f : ex2(mp - m); }
@@ -409,7 +400,12 @@ kv8_attn_kernel(Kv8Dev c, Kv8AttnDev a, AttnGeom g, float *ws) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             float x = z[h][nt][e + 2 * u] * cs;
-                            if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
+                            if (a.cap > 0.0f) {
+                                const float xc = x * inv_cap;
+                                float t = tanh_poly<SPLIT>(xc);
+                                if (__any_sync(0xffffffffu, !(fabsf(xc) <= 0.5f))) t = fabsf(xc) <= 0.5f ? t : tanh_exp(xc);
+                                x = a.cap * t;
+                            }
                             x = fmaf(x, LOG2E, -mrun[nt][e]);
                             z[h][nt][e + 2 * u] = fmaf(-slope, fabsf(dist - (float)(h * KV8_BLOCK + 8 * u)), x);
                         }

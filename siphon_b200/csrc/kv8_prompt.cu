@@ -102,11 +102,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), b, c); }
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t sel) {
     const uint32_t h = prmt(x, 0x64646464u, sel);
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __floats2half2_rn(1152.0f, 1152.0f));
@@ -505,23 +500,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                                                      fabsf(__uint_as_float(v[b >> 1][(b & 1) * 16 + e + 1]))));
                             top = fmaxf(top, bm * cb[b]);
                         }
-                        if (__any_sync(ALL, !(top * cap_in <= 0.25f))) {
-                            // cap tanh x = cap - 2 cap / (1 + e^(2 x)), x = z / cap
+                        if (__any_sync(ALL, !(top * cap_in <= 0.5f))) {
 #pragma unroll
                             for (int b = 0; b < PT_BLOCKS; ++b) {
-                                const float cc = cb[b] * cap_in * (2.0f * LOG2E);
+                                const float cx = cb[b] * cap_in;
 #pragma unroll
                                 for (int e = 0; e < KV8_BLOCK; ++e) {
                                     uint32_t &u = v[b >> 1][(b & 1) * 16 + e];
-                                    u = __float_as_uint(fmaf(-2.0f * cap2, rcp(1.0f + ex2(__uint_as_float(u) * cc)), cap2));
+                                    const float x = __uint_as_float(u) * cx;
+                                    float th = tanh_exp(x);
+                                    if constexpr (SPLIT) th = fabsf(x) <= 0.5f ? tanh_poly<true>(x) : th;
+                                    u = __float_as_uint(cap2 * th);
                                 }
                             }
                         } else {
-                            // Scores below a quarter of the cap, as they mostly are:
-                            // the Taylor series of tanh through x^7 (the next term
-                            // is below 2^-23), two scores at a time on the FMA
-                            // pipe. The form above takes the special-function unit
-                            // twice more per score.
+                            // the polynomial alone (z = cap x), two scores at a time
+                            // on the FMA pipe: the form above
+                            // takes the special-function unit, the busiest here,
+                            // twice more per score
 #pragma unroll
                             for (int b = 0; b < PT_BLOCKS; ++b) {
                                 const uint64_t cx = dup2(cb[b] * cap_in), cw = dup2(cb[b] * LOG2E);
@@ -529,11 +525,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                                 for (int e = 0; e < KV8_BLOCK; e += 2) {
                                     uint32_t &u0 = v[b >> 1][(b & 1) * 16 + e], &u1 = v[b >> 1][(b & 1) * 16 + e + 1];
                                     const uint64_t u = pack2(__uint_as_float(u0), __uint_as_float(u1));
-                                    const uint64_t x = mul2(u, cx), y = mul2(x, x), wz = mul2(u, cw);
-                                    uint64_t g = fma2(y, dup2(-17.0f / 315.0f), dup2(2.0f / 15.0f));
-                                    g = mul2(fma2(g, y, dup2(-1.0f / 3.0f)), y);
+                                    const uint64_t x = mul2(u, cx), y = mul2(x, x), z = mul2(u, cw);
+                                    uint64_t g;
+                                    if constexpr (SPLIT)
+                                        g = fma2(fma2(fma2(y, dup2(TANH4_3), dup2(TANH4_2)), y, dup2(TANH4_1)), y, dup2(TANH4_0));
+                                    else
+                                        g = fma2(fma2(y, dup2(TANH3_2), dup2(TANH3_1)), y, dup2(TANH3_0));
                                     float x0, x1;
-                                    unpack2(fma2(g, wz, wz), x0, x1);
+                                    unpack2(fma2(mul2(z, y), g, z), x0, x1);
                                     u0 = __float_as_uint(x0);
                                     u1 = __float_as_uint(x1);
                                 }
