@@ -315,12 +315,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
     int64_t blk = -1;
     int page = -1;
     float ksc = 0.0f, vsc = 0.0f;
+    // With a distance bias tiles are walked from the last key backwards, so that
+    // the largest scores come first and the maximum stays (640 -> 586 us for two
+    // prompts of 4001 to 6000 tokens, 32 heads of 128 channels); without one,
+    // forwards (backwards cost 700 -> 750 us for one of 8191).
+    auto tile_of = [&](int j) { return a.slopes ? nj - 1 - j : j; };
     auto find_page = [&](int j) {
-        const int b = b0 + j * PT_BLOCKS + lane;
-        page = lane < PT_BLOCKS && b < b1 ? __ldg(a.table + (int64_t)seq * a.max_pages + (b >> (c.page_shift - 4))) : -1;
+        const int b = b0 + tile_of(j) * PT_BLOCKS + lane;
+        page = j < nj && lane < PT_BLOCKS && b < b1 ? __ldg(a.table + (int64_t)seq * a.max_pages + (b >> (c.page_shift - 4))) : -1;
     };
     auto find_blocks = [&](int j) {
-        const int b = b0 + j * PT_BLOCKS + lane;
+        const int b = b0 + tile_of(j) * PT_BLOCKS + lane;
         blk = -1;
         if (lane < PT_BLOCKS && b < b1) {
             if ((unsigned)page >= (unsigned)c.n_pages) {
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, v[q]);
                 const float4 *sj = sc + (j % PT_RING) * PT_BLOCKS;
-                const int k0 = (b0 + j * PT_BLOCKS) * KV8_BLOCK;
+                const int k0 = (b0 + tile_of(j) * PT_BLOCKS) * KV8_BLOCK;
                 const bool masked = k0 < wlo || k0 + PT_KEYS > whi;
                 tmem_wait_all();
 #pragma unroll
