@@ -1417,7 +1417,8 @@ static int check_kv8_attn(const Kv8Dev &c, const sicu_kv8_attn *a, Kv8AttnDev &d
                     (long long)a->max_pages, c.page);
     if (a->max_new < 0 || a->max_new > a->n_tok || a->max_new > a->max_len)
         return fail(SICU_EINVAL, "kv8 attention: up to %lld new tokens of %lld", (long long)a->max_new, (long long)a->n_tok);
-    if (a->max_new * (a->n_head / c.hkv) > INT32_MAX - 1024) return fail(SICU_EINVAL, "kv8 attention: too many rows");
+    if (a->n_tok * a->n_head > INT32_MAX - 65536)
+        return fail(SICU_EINVAL, "kv8 attention: %lld tokens of %d heads: too many rows", (long long)a->n_tok, a->n_head);
     if (a->window < 0) return fail(SICU_EINVAL, "kv8 attention: negative window");
     if (!(a->cap >= 0.0f) || !(a->cap <= 1e30f) || (a->cap > 0.0f && a->cap < 1e-30f))
         return fail(SICU_EINVAL, "kv8 attention: cap %g", (double)a->cap);

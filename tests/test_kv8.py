@@ -106,6 +106,7 @@ def test_attention_checks(so):
     refused(so, call(max_len=129), L.SICU_EINVAL, "lengths")     # 8 pages of 16
     refused(so, call(max_new=4), L.SICU_EINVAL, "new tokens")
     refused(so, call(max_len=1), L.SICU_EINVAL, "new tokens")
+    refused(so, call(n_tok=1 << 30), L.SICU_EINVAL, "too many rows")
     refused(so, call(window=-1), L.SICU_EINVAL, "window")
     refused(so, call(cap=-1.0), L.SICU_EINVAL, "cap")
     refused(so, call(cap=float("nan")), L.SICU_EINVAL, "cap")

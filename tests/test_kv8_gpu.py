@@ -492,3 +492,58 @@ def test_attention_prompt_f32_precision_over_many_keys(sicu):
     # its terms' size, the weights by 2^-22 each
     err = np.linalg.norm(got - want) / np.linalg.norm(want)
     assert err < 2.0 ** -18
+
+
+def test_pool_past_32_bits(sicu):
+    """Pages whose codes begin past 2^32 elements: store, load and both
+    attention kernels reach them (a pool of 5.2 GB for K alone)."""
+    import torch
+    hkv, hd, page, n_pages = 8, 128, 128, 40000
+    bufs = [torch.zeros(n_pages, hkv, page, hd, dtype=torch.int8, device="cuda") for _ in range(2)] + \
+           [torch.zeros(n_pages, hkv, page // 16, device="cuda") for _ in range(2)]
+    cache = L.kv8_cache(*bufs, n_pages, page, hkv, hd)
+    rng = np.random.default_rng(8)
+    pages = [39999, 12, 38001]
+    n = 300
+    slot = np.array([pages[p // page] * page + p % page for p in range(n)], np.int64)
+    x = rng.standard_normal((2, n, hkv, hd)).astype(np.float32)
+    small = [R.Cache(3, hkv, page, hd) for _ in range(2)]            # the same rows in pages 0, 1, 2
+    for c, v in zip(small, x):
+        c.store(v, np.arange(n, dtype=np.int64))
+    sicu.kv8_store(cache, L.T_F32, dev(x[0]), dev(x[1]), dev(slot), n)
+    out = [torch.empty(n, hkv, hd, device="cuda") for _ in range(2)]
+    sicu.kv8_load(cache, L.T_F32, dev(slot), n, *out)
+    for got, c in zip(out, small):
+        assert np.allclose(host(got), c.load(np.arange(n)), rtol=2.0 ** -22, atol=0)
+    for new in (1, 60):
+        q = rng.standard_normal((new, 16, hd)).astype(np.float32)
+        want, _ = R.attention(q.astype(np.float64), *small, np.array([[0, 1, 2]], np.int32), [n], [0, new], 0.088)
+        o = torch.empty(new, 16, hd, device="cuda")
+        d_table, d_len, d_cu = i32([pages]), i32([n]), i32([0, new])
+        at = L.kv8_attn(L.T_F32, 16, new, d_table, 3, d_len, d_cu, 1, new, n, 0.088)
+        ws = torch.empty(max(sicu.kv8_attention_ws(cache, at), 16), dtype=torch.uint8, device="cuda")
+        sicu.kv8_attention(cache, at, dev(q), o, ws)
+        # scores of a few units in f32, values of 4 at most
+        assert np.abs(host(o) - want).max() < 4 * 2.0 ** -17
+    assert sicu.status() == 0
+
+
+def test_positions_past_the_rope_tables_are_reported(sicu):
+    import torch
+    rng = np.random.default_rng(9)
+    k, v, bufs, cache = make_cache(8, 2, 16, 64, rng)
+    cos, sin = R.rope_tables(40, 64)
+    d_cos, d_sin = dev(cos), dev(sin)
+    rope = L.rope(d_cos, d_sin, 40, 64)
+    x = rng.standard_normal((3, 2, 64)).astype(np.float32)
+    sicu.kv8_store(cache, L.T_F32, dev(x), dev(x), dev(np.arange(3, dtype=np.int64)), 3, pos=i32([39, 40, -1]), rope=rope)
+    assert sicu.status() == L.STATUS_BAD_PLAN
+    for new in (1, 50):
+        q = rng.standard_normal((new, 8, 64)).astype(np.float32)
+        out = torch.zeros(new, 8, 64, device="cuda")
+        d_table, d_len, d_cu = i32([np.arange(8)]), i32([60]), i32([0, new])
+        at = L.kv8_attn(L.T_F32, 8, new, d_table, 8, d_len, d_cu, 1, new, 60, 0.125, rope=rope)
+        ws = torch.empty(max(sicu.kv8_attention_ws(cache, at), 16), dtype=torch.uint8, device="cuda")
+        sicu.kv8_attention(cache, at, dev(q), out, ws)
+        assert np.isfinite(host(out)).all()
+        assert sicu.status() == L.STATUS_BAD_PLAN
