@@ -26,7 +26,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr int AT_WARPS = 4;
-constexpr int AT_MOST = 32;
+constexpr int AT_MOST = 64;
 // A new maximum rescales the accumulator only when it passes the running one
 // by 2^8: weights stay below 2^8 and f16 carries them as precisely.
 constexpr float AT_LAZY = 8.0f;
@@ -661,28 +661,37 @@ __global__ void __launch_bounds__(COMB_WARPS * 32) kv8_combine_kernel(Kv8Dev c, 
 }
 
 // The rows (query heads of one KV head x new tokens) up to which a request
-// runs here; longer ones on the tensor-memory kernel, whose 128-row tiles few
-// rows would leave empty and whose keys are not split over CTAs. A single
+// runs here; longer ones on the tensor-memory kernel, whose CTAs of 128 to 256
+// rows each walk all the keys. Here time grows with the rows, there it does
+// not, but only requests x KV heads fill the GPU. 16 requests of 4250 tokens at
+// the Llama-3-8B shape (128 CTAs there): 64 rows 222 us here, 210 there; 128
+// rows 363 and 217. Two of them (16 CTAs): 128 rows 56 and 132. Hence 64 rows,
+// and in proportion more, up to 256, where those CTAs leave SMs idle. A single
 // request runs on one kernel.
-int attn_most(const Kv8Dev &c, const Kv8AttnDev &a) {
+int attn_limit(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
+    const int64_t share = num_sms / ((int64_t)a.n_seq * c.hkv);
+    return AT_MOST * (int)(share < 1 ? 1 : share > 4 ? 4 : share);
+}
+int attn_most(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     const int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
-    if (!kv8_prompt_supported(c.hd) || rows <= AT_MOST) return INT_MAX;
-    return a.n_seq == 1 ? 0 : AT_MOST;
+    const int limit = attn_limit(c, a, num_sms);
+    if (!kv8_prompt_supported(c.hd) || rows <= limit) return INT_MAX;
+    return a.n_seq == 1 ? 0 : limit;
 }
 
 // n tiles per CTA: the rows of a request's longest piece, up to 32 (16 with
 // 256 channels, whose accumulator would not fit the registers). In a step that
 // mixes prompts with single tokens, those of one token.
-int attn_nt(const Kv8Dev &c, const Kv8AttnDev &a) {
+int attn_nt(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
     const int group = a.n_head / c.hkv;
-    const int64_t rows = attn_most(c, a) == AT_MOST ? group : (int64_t)a.max_new * group;
+    const int64_t rows = attn_most(c, a, num_sms) != INT_MAX ? group : (int64_t)a.max_new * group;
     return rows <= 8 ? 1 : rows <= 16 || c.hd == 256 ? 2 : 4;
 }
 
 AttnGeom attn_geom(const Kv8Dev &c, const Kv8AttnDev &a, int num_sms) {
-    const int nt = attn_nt(c, a), R = 8 * nt;
+    const int nt = attn_nt(c, a, num_sms), R = 8 * nt;
     AttnGeom g{};
-    g.most = attn_most(c, a);
+    g.most = attn_most(c, a, num_sms);
     if (g.most == 0) return g;               // no request runs here
     int64_t rows = (int64_t)a.max_new * (a.n_head / c.hkv);
     if (rows > g.most) rows = g.most;
@@ -734,8 +743,8 @@ int launch_typed(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float 
 }
 
 template <typename T, int HD>
-int launch_hd(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
-    switch (attn_nt(c, a)) {
+int launch_hd(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, int nt, float *ws, cudaStream_t st) {
+    switch (nt) {
         case 1: return launch_typed<T, HD, 1>(c, a, g, ws, st);
         case 2: return launch_typed<T, HD, 2>(c, a, g, ws, st);
         default:
@@ -745,12 +754,12 @@ int launch_hd(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws
 }
 
 template <typename T>
-int launch_t(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, float *ws, cudaStream_t st) {
+int launch_t(const Kv8Dev &c, const Kv8AttnDev &a, const AttnGeom &g, int nt, float *ws, cudaStream_t st) {
     switch (c.hd) {
-        case 64: return launch_hd<T, 64>(c, a, g, ws, st);
-        case 96: return launch_hd<T, 96>(c, a, g, ws, st);
-        case 128: return launch_hd<T, 128>(c, a, g, ws, st);
-        case 256: return launch_hd<T, 256>(c, a, g, ws, st);
+        case 64: return launch_hd<T, 64>(c, a, g, nt, ws, st);
+        case 96: return launch_hd<T, 96>(c, a, g, nt, ws, st);
+        case 128: return launch_hd<T, 128>(c, a, g, nt, ws, st);
+        case 256: return launch_hd<T, 256>(c, a, g, nt, ws, st);
         default: return -3;
     }
 }
@@ -770,8 +779,9 @@ int launch_kv8_attention(const Kv8Dev &c, const Kv8AttnDev &a, bool f16, void *w
         if (const int rc = launch_kv8_prompt(c, a, f16, g.most, num_sms, st)) return rc;
         if (g.most == 0) return 0;
     }
-    return f16 ? launch_t<__half>(c, a, g, static_cast<float *>(ws), st)
-               : launch_t<float>(c, a, g, static_cast<float *>(ws), st);
+    const int nt = attn_nt(c, a, num_sms);
+    return f16 ? launch_t<__half>(c, a, g, nt, static_cast<float *>(ws), st)
+               : launch_t<float>(c, a, g, nt, static_cast<float *>(ws), st);
 }
 
 }  // namespace sicu

@@ -547,3 +547,21 @@ def test_positions_past_the_rope_tables_are_reported(sicu):
         sicu.kv8_attention(cache, at, dev(q), out, ws)
         assert np.isfinite(host(out)).all()
         assert sicu.status() == L.STATUS_BAD_PLAN
+
+
+@pytest.mark.parametrize("n_head,hkv,hd", [(8, 2, 64), (10, 2, 128)])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("mask", ["none", "cap", "steep cap", "slopes", "window", "prefix", "first", "all"])
+def test_attention_masks_over_many_rows(sicu, n_head, hkv, hd, f16, mask):
+    """Requests of several hundred rows (query heads x tokens), more than one
+    tile of the tensor-memory kernel, next to short ones: full and partly
+    filled tiles, spans that begin inside a block, rows and whole requests that
+    see nothing, scores on both sides of half the cap."""
+    past, fresh = [0, 40, 300, 7], [150, 1, 70, 133]
+    lens = [p + f for p, f in zip(past, fresh)]
+    kw = {"cap": {"cap": 200.0}, "steep cap": {"cap": 3.0}, "slopes": {"slopes": True}, "window": {"window": 37},
+          "prefix": {"prefix": [lens[0], 0, 320, lens[3] // 2]}, "first": {"first": [100, 41, lens[2], 3]}, "none": {},
+          "all": {"cap": 20.0, "slopes": True, "window": 61, "prefix": [20, 0, 340, 0], "first": [100, 0, 333, 140]}}[mask]
+    got, want = attend(sicu, n_head, hkv, hd, 16, past, fresh, f16=f16, neox=f16, seed=3, **kw)
+    if mask == "first":
+        assert (got[:100] == 0).all() and (got[151:221] == 0).all() and got[100].any()
