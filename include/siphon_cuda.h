@@ -570,10 +570,11 @@ SICU_API int sicu_kv8_load(const sicu_kv8 *cache, uint32_t type, const int64_t *
  * softmax(z)_j v_j; a row that sees no key is 0. q and out: type SICU_T_F32 or
  * SICU_T_F16, n_head * head_dim values per token, q_stride / out_stride
  * elements apart, 16-byte aligned; q is rotated at its position when rope is
- * given and left as it is in memory. Sums and maxima are f32; f32 results
- * agree with a computation in f32, f16 ones are rounded once at the end (the
- * softmax weights pass through f16 in between). max_new and max_len bound the
- * requests' new tokens and lengths (host values). */
+ * given and left as it is in memory. Sums and maxima are f32. f32 results:
+ * single tokens as close to 64 bits as a computation in f32, prompts within a
+ * few 1e-6 (the tensor cores' f32 sums drop bits); f16 ones are rounded once at
+ * the end (the softmax weights pass through f16 in between). max_new and
+ * max_len bound the requests' new tokens and lengths (host values). */
 typedef struct sicu_kv8_attn {
     uint32_t type;
     int32_t n_head;

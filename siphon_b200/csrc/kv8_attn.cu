@@ -16,8 +16,11 @@
 //                      parts (hi + lo, 22 bits) for f32 callers, rounded once
 //                      to f16 (2^-11, the size of the output's own rounding)
 //                      for f16 callers
-// Maxima, sums and the output stay in f32. Bound by issue: expanding V and the
-// weights cost about as many instructions as DRAM gives time for at its rate.
+// Maxima, sums and the output stay in f32. Measured, 64 requests of 4250 tokens
+// on average, 32 heads of 128 over 8 KV heads, f32 q (523 MB of cache): 102 us
+// for this kernel, 5.1 TB/s of the 6.5 a copy reaches. Bound by latency and
+// issue: some 330 instructions per 16 keys (a third expand V's codes) at three
+// warps per scheduler, 45 % of the issue slots taken.
 #include "kv8.cuh"
 #include "tc.cuh"
 

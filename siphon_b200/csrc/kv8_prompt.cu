@@ -18,8 +18,14 @@
 // q enters as two f16 parts (hi + lo; a row of f16 values that is not rotated
 // is exact in one), so scores agree with an f32 computation; f32 callers'
 // weights do too, f16 callers' are rounded once to f16. That makes 3 (f32: 4)
-// MMA passes of the 2 that the operation's flops count, the bound of the
-// kernel at 128 channels: 2/3 (1/2) of the tensor cores' rate.
+// MMA passes of the 2 that the operation's flops count: at 128 channels at most
+// 2/3 (1/2) of the tensor cores' rate. Measured, 8191 tokens of 32 heads of 128
+// over 8 KV heads, f16, causal: 0.70 to 0.72 ms, 770 TFLOP/s of the operation,
+// 1150 of MMAs where the cores reach 1627 (0.66 ms without RoPE, whose rotated
+// q needs its second part). A tile pair takes some 4600 cycles, 3072 of them
+// MMAs; the rest is the hand-over from scores to weights (one thread per row:
+// 128 exponentials are 1024 cycles of the special-function unit per tile), and
+// a CTA's first and last steps are some 20 K cycles.
 #include "kv8.cuh"
 #include "tc.cuh"
 
@@ -39,13 +45,13 @@ constexpr int PT_BUF = 3;             // f16 tiles: K and V of successive key ti
 constexpr int PT_RING = 4;            // tiles whose scales are kept
 // The tensor cores drop bits of an f32 sum at every step of 16 keys, always
 // toward zero: some 1.2e-8 of it, and twice the steps with weights in two
-// parts. For f32 callers the output's sums start anew every 16 tiles, the
-// finished ones added up in the output rows: relative error 2.9e-6 for an
-// 8191-token prompt at the Llama-3-8B shape, where it was 6.2e-6 and growing with
-// the context (an f32 computation's is 1.1e-6), for 12 % of that prompt's time
-// (861 -> 964 us). f16 callers' results stay below their own rounding up to
-// 128 K keys without.
-constexpr int PT_FLUSH = 16;
+// parts. For f32 callers the output's sums start anew every 8 tiles, the
+// finished ones added up in the output rows: relative error 1.8e-6 for an
+// 8191-token prompt at the Llama-3-8B shape (an f32 computation's 1.1e-6) for
+// 1.18 ms. Every 16 tiles 2.9e-6 and 1.02 ms, every 4 1.1e-6 and 1.52 ms, never
+// 6.2e-6, growing with the context, and 0.9 ms. f16 callers' results stay below
+// their own rounding up to 128 K keys without.
+constexpr int PT_FLUSH = 8;
 
 // Barriers. The converters fill the three tile buffers in the order K0 V0 K1
 // V1 ...: V of tile j then waits only for the scores of tile j (K's release),
