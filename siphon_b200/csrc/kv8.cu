@@ -223,10 +223,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_release_kernel(const int32_t
 // and the result does not depend on any order. The slots and positions a CTA
 // needs are read at once at its start, and a row's table entries with its
 // values: two memory latencies per block, where one warp per block and its
-// reads in the order of use took four and half the warps (59 -> 49 us for 15,900
-// tokens of 8 heads of 128, f32, 165 MB). Bound by DRAM bytes for prompts and by
-// those latencies for single tokens.
+// reads in the order of use took four and half the warps (59 -> 47 us for 15,900
+// tokens of 8 heads of 128, f32, 165 MB). A CTA's two pairs take K of one run
+// and V of the next in turn, since K's rotation is more work (47 -> 44 us).
+// Prompts are bound by issue (half the cycles) and those latencies at 20 warps per
+// SM, 3.8 TB/s; single tokens by the latencies.
 constexpr int STORE_WARPS = 4;
+static_assert(STORE_WARPS == 4, "one pair of warps for K, one for V");
 // smallest magnitude worth a scale: below it 1 / scale would leave f32's range
 constexpr float KV8_TINY = 1.92592994e-34f;     // 2^-112
 
@@ -263,12 +266,11 @@ __global__ void __launch_bounds__(STORE_WARPS * 32, HD <= 128 ? 5 : 3) kv8_store
     int64_t prev = __shfl_up_sync(0xffffffffu, sa, 1);
     if (lane == 0) prev = sp;
     const bool opens = lane < chunk && sa >= 0 && (prev < 0 || (prev >> 4) != (sa >> 4));
-    const uint32_t starts = __ballot_sync(0xffffffffu, opens);
-    const int jobs = 2 * __popc(starts);
-    int parity = 0;
-    for (int j = pair; j < jobs; j += STORE_WARPS / 2, parity ^= 1) {
-        const bool is_v = j & 1;
-        const int i0 = __fns(starts, 0, (j >> 1) + 1);
+    uint32_t starts = __ballot_sync(0xffffffffu, opens);
+    // one pair of warps takes K of a run and the other V, in turn
+    for (int parity = 0; starts; starts &= starts - 1, parity ^= 1) {
+        const bool is_v = (pair ^ parity) != 0;
+        const int i0 = __ffs(starts) - 1;
         const int64_t r0 = c0 + i0;
         // the run: rows r0 .. r0 + n - 1 in one block; lane i knows row i
         const int from = i0 + lane;
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(STORE_WARPS * 32, HD <= 128 ? 5 : 3) kv8_store
 // ---- load ----------------------------------------------------------------------------
 // Rows of the cache as values: code * scale. A CTA takes eight rows; a lane four
 // codes at a time, so that a warp writes 512 consecutive bytes (16 codes per
-// lane, four strided stores, wrote half sectors: 41 us against 33 for 15,900
+// lane, four strided stores, wrote half sectors: 41 us against 32 for 15,900
 // rows of 8 heads of 128, f32, 163 MB), K's and V's read before either is written.
 // Bound by the bytes of the values written.
 constexpr int LOAD_ROWS = 8;
@@ -415,27 +417,32 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(Kv8Dev c, const int64_t *
     const unsigned per_head = c.hd / 4, words = c.hkv * per_head;
     const int64_t t0 = (int64_t)blockIdx.x * LOAD_ROWS;
     const unsigned rows = (unsigned)(n_tok - t0 < LOAD_ROWS ? n_tok - t0 : LOAD_ROWS);
+    // a thread keeps its words (heads and channels) over the rows
+    const unsigned across = words < 256 ? words : 256, ry = threadIdx.x / across, step = 256 / across;
+    if (ry >= step) return;
+    for (unsigned w = threadIdx.x - ry * across; w < words; w += across) {
+        const unsigned head = w / per_head, e = w - head * per_head;
+        T *const dk = k + t0 * words * 4 + w * 4, *const dv = v + t0 * words * 4 + w * 4;
 #pragma unroll 4
-    for (unsigned i = threadIdx.x; i < rows * words; i += 256) {
-        const unsigned r = i / words, p = i - r * words, head = p / per_head, e = p - head * per_head;
-        const int64_t s = __ldg(slot + t0 + r), pg = s >> c.page_shift;
-        const int64_t dst = ((t0 + r) * c.hkv + head) * c.hd + e * 4;
-        uint32_t wk = 0, wv = 0;
-        float sk = 0.0f, sv = 0.0f;
-        if (s >= 0 && pg < c.n_pages) {
-            const int64_t blk = kv8_block(c, (int)pg, head, (int)(s & (c.page - 1)) >> 4);
-            const int64_t at = (blk * KV8_BLOCK + (s & (KV8_BLOCK - 1))) * c.hd + e * 4;
-            wk = *reinterpret_cast<const uint32_t *>(c.k + at);
-            wv = *reinterpret_cast<const uint32_t *>(c.v + at);
-            sk = c.ks[blk];
-            sv = c.vs[blk];
-        } else if (s >= 0) {
-            atomicOr(status, STATUS_BAD_PLAN);
+        for (unsigned r = ry; r < rows; r += step) {
+            const int64_t s = __ldg(slot + t0 + r), pg = s >> c.page_shift;
+            uint32_t wk = 0, wv = 0;
+            float sk = 0.0f, sv = 0.0f;
+            if (s >= 0 && pg < c.n_pages) {
+                const int64_t blk = kv8_block(c, (int)pg, head, (int)(s & (c.page - 1)) >> 4);
+                const int64_t at = (blk * KV8_BLOCK + (s & (KV8_BLOCK - 1))) * c.hd + e * 4;
+                wk = __ldg(reinterpret_cast<const uint32_t *>(c.k + at));
+                wv = __ldg(reinterpret_cast<const uint32_t *>(c.v + at));
+                sk = __ldg(c.ks + blk);
+                sv = __ldg(c.vs + blk);
+            } else if (s >= 0) {
+                atomicOr(status, STATUS_BAD_PLAN);
+            }
+            store4(dk + (int64_t)r * words * 4, (float)(int8_t)wk * sk, (float)(int8_t)(wk >> 8) * sk,
+                   (float)(int8_t)(wk >> 16) * sk, (float)(int8_t)(wk >> 24) * sk);
+            store4(dv + (int64_t)r * words * 4, (float)(int8_t)wv * sv, (float)(int8_t)(wv >> 8) * sv,
+                   (float)(int8_t)(wv >> 16) * sv, (float)(int8_t)(wv >> 24) * sv);
         }
-        store4(k + dst, (float)(int8_t)wk * sk, (float)(int8_t)(wk >> 8) * sk, (float)(int8_t)(wk >> 16) * sk,
-               (float)(int8_t)(wk >> 24) * sk);
-        store4(v + dst, (float)(int8_t)wv * sv, (float)(int8_t)(wv >> 8) * sv, (float)(int8_t)(wv >> 16) * sv,
-               (float)(int8_t)(wv >> 24) * sv);
     }
 }
 
