@@ -150,6 +150,9 @@ class PagedPath(MatrixPath):
     def retire(self, stream, requests) -> None:
         """The requests ended: their pages become free, their places empty."""
         import torch
+        requests = list(requests)
+        if any(not 0 <= i < self.max_seqs for i in requests):
+            raise ValueError(f"requests {requests} of {self.max_seqs}")
         drop = torch.zeros(self.max_seqs, dtype=torch.int32)
         for i in requests:
             drop[i] = 1

@@ -86,3 +86,13 @@ def test_step_argument_errors(tmp_path):
         q.step(_Stream(), [17, 17, 0], list(range(34)))
     with pytest.raises(ValueError, match="no request"):
         q.decode(_Stream())
+
+
+@pytest.mark.parametrize("requests", [[0, 3], [-1], [1, -3]])
+def test_retire_refuses_places_it_does_not_have(tmp_path, requests):
+    p, rec = make(tmp_path)
+    p.step(_Stream(), [5, 1, 20], list(range(26)))
+    rec.calls.clear()
+    with pytest.raises(ValueError):
+        p.retire(_Stream(), requests)
+    assert not rec.calls and p.len_host == [5, 1, 20]
