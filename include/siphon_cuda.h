@@ -530,7 +530,8 @@ typedef struct sicu_rope_tables {
  * that does not fit places nothing (cu all 0, slots all -1, len = past,
  * n_free_out = n_free): SICU_STATUS_NO_PAGES when the stack is too short,
  * SICU_STATUS_BAD_PLAN for a negative length, a request past max_pages or more
- * than n_tok tokens. */
+ * than n_tok tokens. A token whose page id is outside the pool gets slot -1 and
+ * sets SICU_STATUS_BAD_PLAN. */
 SICU_API int sicu_kv8_plan(const int32_t *past, const int32_t *fresh, int64_t n_seq, int32_t page, int32_t *table,
                            int64_t max_pages, const int32_t *free_pages, int64_t n_pages, const int32_t *n_free,
                            int32_t *n_free_out, int64_t n_tok, int32_t *cu, int32_t *len, int64_t *slot, int32_t *pos,

@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_plan_kernel(Kv8PlanLaunch L)
                 const int p = past[i] + t - cu[i], col = p >> sh, held = (past[i] + pm) >> sh;
                 const int page = col < held ? L.table[(int64_t)i * L.max_pages + col]
                                             : L.free_pages[n_free - 1 - (tk[i] + col - held)];
-                s[e] = ((int64_t)page << sh) + (p & pm);
+                if ((unsigned)page < (uint64_t)L.n_pages) s[e] = ((int64_t)page << sh) + (p & pm);
+                else atomicOr(L.status, STATUS_BAD_PLAN);
                 ps[e] = p;
             }
         }

@@ -22,7 +22,7 @@
 // 2/3 (1/2) of the tensor cores' rate. Measured, 8191 tokens of 32 heads of 128
 // over 8 KV heads, f16, causal: 0.70 to 0.72 ms, 770 TFLOP/s of the operation,
 // 1150 of MMAs where the cores reach 1627 (0.66 ms without RoPE, whose rotated
-// q needs its second part). A tile pair takes some 4600 cycles, 3072 of them
+// q needs its second part). A tile pair takes some 4600 cycles, 3.1 K of them
 // MMAs; the rest is the hand-over from scores to weights (one thread per row:
 // 128 exponentials are 1024 cycles of the special-function unit per tile), and
 // a CTA's first and last steps are some 20 K cycles.

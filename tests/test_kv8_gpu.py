@@ -92,6 +92,21 @@ def test_plan_places_nothing_when_it_does_not_fit(sicu, why):
     assert (host(slot) == -1).all() and (host(pos) == 0).all() and host(out)[0] == n_free
 
 
+def test_plan_leaves_out_tokens_of_pages_outside_the_pool(sicu):
+    import torch
+    # request 0 goes on in a held page, 1 takes the stack's top two, 2 the one below
+    table = np.array([[-3, 0], [0, 0], [0, 0], [7, 0]], np.int32)
+    stack = i32([0, 1, 2, 3, 12, 5, 10, 0, 0, 0])     # ids 0 .. 9; n_free 7: takes 10, 5, then 12
+    cu, length = torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    slot = torch.zeros(24, dtype=torch.int64, device="cuda")
+    pos = torch.zeros(24, dtype=torch.int32, device="cuda")
+    sicu.kv8_plan(i32([3, 0, 0, 2]), i32([1, 18, 2, 1]), 4, 16, dev(table), 2, stack, 10, i32([7]), i32([0]), 24, cu,
+                  length, slot, pos)
+    assert sicu.status() == L.STATUS_BAD_PLAN
+    assert host(slot).tolist() == [-1] + [-1] * 16 + [80, 81] + [-1, -1] + [7 * 16 + 2] + [-1, -1]
+    assert host(length).tolist() == [4, 18, 2, 3] and host(cu).tolist() == [0, 1, 19, 21, 22]
+
+
 def test_release_and_reuse(sicu):
     page, width = 16, 4
     table = np.arange(20, dtype=np.int32).reshape(5, width)
