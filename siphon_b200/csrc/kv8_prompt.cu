@@ -51,7 +51,15 @@ constexpr int PT_RING = 4;            // tiles whose scales are kept
 // 1.18 ms. Every 16 tiles 2.9e-6 and 1.02 ms, every 4 1.1e-6 and 1.52 ms, never
 // 6.2e-6, growing with the context, and 0.9 ms. f16 callers' results stay below
 // their own rounding up to 128 K keys without.
+//
+// What a finished sum of n tiles has lost lies between nothing (all of it came
+// last, or what came later added exact zeros) and twice what a sum that grew
+// evenly has, so it is raised by n PT_LOST, some three quarters of the latter:
+// the same prompt 1.2e-6, six chunks of 1 to 1500 tokens 1.7e-6 -> 1.1e-6.
+// Raised by all of it (1.7e-7) these had 1.0e-6, but prompts whose distance bias
+// lets few tiles count 1.1e-6 instead of 0.9e-6 (0.86e-6 unraised).
 constexpr int PT_FLUSH = 8;
+constexpr float PT_LOST = 1.3e-7f;
 
 // Barriers. The converters fill the three tile buffers in the order K0 V0 K1
 // V1 ...: V of tile j then waits only for the scores of tile j (K's release),
@@ -465,6 +473,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                     // S of this tile is complete, so every product before it is
                     if (j > 0 && j % PT_FLUSH == 0) {
                         float *dst = reinterpret_cast<float *>(out) + row_at;
+                        constexpr float UP = 1.0f + PT_FLUSH * PT_LOST;
 #pragma unroll 1
                         for (int q = 0; q < HD; q += 16) {
                             uint32_t w[16];
@@ -475,10 +484,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
                                 for (int e = 0; e < 16; e += 4) {
                                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                                     if (j > PT_FLUSH) x = *reinterpret_cast<const float4 *>(dst + q + e);
-                                    x.x = fmaf(x.x, kept, __uint_as_float(w[e]));
-                                    x.y = fmaf(x.y, kept, __uint_as_float(w[e + 1]));
-                                    x.z = fmaf(x.z, kept, __uint_as_float(w[e + 2]));
-                                    x.w = fmaf(x.w, kept, __uint_as_float(w[e + 3]));
+                                    x.x = fmaf(x.x, kept, __uint_as_float(w[e]) * UP);
+                                    x.y = fmaf(x.y, kept, __uint_as_float(w[e + 1]) * UP);
+                                    x.z = fmaf(x.z, kept, __uint_as_float(w[e + 2]) * UP);
+                                    x.w = fmaf(x.w, kept, __uint_as_float(w[e + 3]) * UP);
                                     *reinterpret_cast<float4 *>(dst + q + e) = x;
                                 }
                             }
@@ -659,7 +668,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
             }
             if (ok && __all_sync(ALL, pt_wait<true>(bar(B_OUT), 0, abort_flag, a.status))) {
                 tc_fence_after();
-                const float f = l == 0.0f ? 0.0f : __fdiv_rn(*vref_sm, l);
+                float f = l == 0.0f ? 0.0f : __fdiv_rn(*vref_sm, l), kept_up = kept;
+                if constexpr (SPLIT) {
+                    // the last tiles' sums raised, not the rows written before
+                    const float up = 1.0f + (float)((nj - 1) % PT_FLUSH + 1) * PT_LOST;
+                    f *= up;
+                    kept_up = __fdividef(kept, up);
+                }
                 // through this warp's part of q's shared memory (every product
                 // has ended), so that rows are written whole: 16-byte units,
                 // turned by the row against bank conflicts
@@ -677,10 +692,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv8_prompt_kernel(const __grid_
 #pragma unroll
                             for (int e = 0; e < 32; e += 4) {
                                 const float4 x = *reinterpret_cast<const float4 *>(src + e);
-                                w[e] = __float_as_uint(fmaf(x.x, kept, __uint_as_float(w[e])));
-                                w[e + 1] = __float_as_uint(fmaf(x.y, kept, __uint_as_float(w[e + 1])));
-                                w[e + 2] = __float_as_uint(fmaf(x.z, kept, __uint_as_float(w[e + 2])));
-                                w[e + 3] = __float_as_uint(fmaf(x.w, kept, __uint_as_float(w[e + 3])));
+                                w[e] = __float_as_uint(fmaf(x.x, kept_up, __uint_as_float(w[e])));
+                                w[e + 1] = __float_as_uint(fmaf(x.y, kept_up, __uint_as_float(w[e + 1])));
+                                w[e + 2] = __float_as_uint(fmaf(x.z, kept_up, __uint_as_float(w[e + 2])));
+                                w[e + 3] = __float_as_uint(fmaf(x.w, kept_up, __uint_as_float(w[e + 3])));
                             }
                         }
                     }
